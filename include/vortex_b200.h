@@ -33,7 +33,7 @@ typedef enum vtx_status {
     VTX_ERR_UNSUPPORTED = -2,  /* legal request this build has no kernel for           */
     VTX_ERR_ALIGNMENT = -3,    /* pointer or stride not aligned as the kernel needs    */
     VTX_ERR_LAUNCH = -4,       /* CUDA reported an error at launch                     */
-    VTX_ERR_DEVICE = -5        /* a kernel set its status word (bounded wait ran out)  */
+    VTX_ERR_DEVICE = -5        /* a kernel set its status word (bounded wait ran out, no page for a token) */
 } vtx_status;
 
 enum { VTX_F32 = 0, VTX_BF16 = 1, VTX_F16 = 2 };
@@ -60,13 +60,13 @@ enum { VTX_BIAS_NONE = 0, VTX_BIAS_ADD = 1, VTX_BIAS_GATED = 2 /* + bias[d] * kv
 size_t vtx_last_error(char* buf, size_t len);
 /* ABI version of this header: major * 1000 + minor.  vtx_abi_version() returns the value the library was
  * built with; a binding compares the two (same major, library minor >= the minor it was written for). */
-#define VTX_ABI_VERSION 1006
+#define VTX_ABI_VERSION 1007
 int64_t vtx_abi_version(void);
 /* sizeof() of the parameter structs in declaration order (0 = vtx_featurizer_params, ...),
  * -1 past the end; lets a binding verify that its mirror of a struct has the same size. */
 int64_t vtx_struct_size(int64_t which);
 /* Reads and clears the device status word that kernels set when one of their bounded waits
- * (mbarrier / TMA completion) ran out.  Synchronous (a small device-to-host copy); meant to be
+ * (mbarrier / TMA completion) ran out, or when a block table gave them no page for a token.  Synchronous (a small device-to-host copy); meant to be
  * called after the stream was synchronised.  Returns VTX_OK or VTX_ERR_DEVICE. */
 int vtx_device_status(void);
 /* Kernels launched by this library since it was loaded (all entry points, all threads).  A caller that wants the
@@ -472,6 +472,112 @@ typedef struct vtx_decode_layer_params {
     int64_t io_dtype;
 } vtx_decode_layer_params;
 int vtx_decode_layer(const vtx_decode_layer_params* p, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention layers between the Hyena layers: positions, a paged cache of keys
+ * and values, one new token against it.
+ *
+ * vtx_qk_norm_rotary_fwd: queries q [B,L,Hq,D] and keys k [B,L,Hk,D] (element
+ * strides, unit stride over D; Hq or Hk may be 0) -> q_out, k_out of the same
+ * shapes and dtype.  With a weight [D] a head is first divided by its root
+ * mean square: u = w x / sqrt(mean x^2 + eps); without one u = x.  Then pair
+ * i < rot / 2 turns by t = position * inv_freq[i]:
+ *   y_a = scale (u_a cos t - u_b sin t),  y_b = scale (u_a sin t + u_b cos t)
+ * with (a, b) = (2i, 2i+1) when interleaved, else (i, i + rot/2); dimensions
+ * from rot on keep u.  Positions are int32 or int64 (any sign, |p| < 2^31),
+ * inv_freq fp32 or fp64 [rot/2]; the angle is formed in fp64, all else in
+ * fp32, one rounding at the end.  Outputs may be the inputs themselves (same
+ * strides), not overlap them otherwise.  D <= 512.
+ * The reference rotates in vortex/ops/embedding/rotary.py:12 (no norm).
+ * ------------------------------------------------------------------------ */
+typedef struct vtx_rotary_params {
+    const void* q;  int64_t q_stride_b, q_stride_l, q_stride_h;
+    const void* k;  int64_t k_stride_b, k_stride_l, k_stride_h;
+    void* q_out;    int64_t q_out_stride_b, q_out_stride_l, q_out_stride_h;
+    void* k_out;    int64_t k_out_stride_b, k_out_stride_l, k_out_stride_h;
+    const void* positions; int64_t positions_i64, pos_stride_b, pos_stride_l;   /* [B,L] */
+    const void* inv_freq;  int64_t inv_freq_f64, rot;
+    const void* q_weight;  int64_t q_weight_dtype;   /* [D] or NULL */
+    const void* k_weight;  int64_t k_weight_dtype;   /* [D] or NULL */
+    double scale, eps;
+    int64_t interleaved;
+    int64_t B, L, Hq, Hk, D;
+    int64_t io_dtype;
+} vtx_rotary_params;
+int vtx_qk_norm_rotary_fwd(const vtx_rotary_params* p, void* stream);
+
+/* Backward of the same call.  fwd: its parameters, with fwd.q_out / fwd.k_out (and their strides) receiving the gradients of
+ * q and k.  dq_out / dk_out: the gradients of its outputs.  dq_weight / dk_weight [D] in the weights' dtypes, where there are
+ * weights.  The weights' gradients are summed in fp32 in a fixed order: equal calls give equal bits.  scratch:
+ * vtx_qk_norm_rotary_bwd_scratch_bytes(&fwd) bytes (0 without weights, q and k are then not read). */
+typedef struct vtx_rotary_bwd_params {
+    vtx_rotary_params fwd;
+    const void* dq_out; int64_t dq_out_stride_b, dq_out_stride_l, dq_out_stride_h;
+    const void* dk_out; int64_t dk_out_stride_b, dk_out_stride_l, dk_out_stride_h;
+    void* dq_weight; void* dk_weight;
+    void* scratch;
+} vtx_rotary_bwd_params;
+int64_t vtx_qk_norm_rotary_bwd_scratch_bytes(const vtx_rotary_params* p);
+int vtx_qk_norm_rotary_bwd(const vtx_rotary_bwd_params* p, void* stream);
+
+/* vtx_rotary_append: vtx_qk_norm_rotary_fwd on the queries and keys of new tokens, with the keys, and the values v
+ * [B,L,Hk,D] as they are, stored in the pages of a cache instead of k_out (not read): token t of the B*L (in that order)
+ * belongs to row s = seq_ids[t] of the block table (s = t where seq_ids is NULL) and goes to page
+ * block_table[s][position / page_size], slot position % page_size.  Pools [num_pages, page_size, Hk, D] by element strides.
+ * A token of a negative position is padding and stored nowhere.  One that the table gives no page (its position behind the
+ * table's width, its row outside the table, an entry outside 0 .. num_pages-1) is not stored either and sets the device
+ * status word.  Two tokens of one call must not share a slot.  No other byte of the pools is written. */
+typedef struct vtx_rotary_append_params {
+    vtx_rotary_params rot;
+    const void* v;  int64_t v_stride_b, v_stride_l, v_stride_h;
+    void* k_pages;  int64_t k_stride_page, k_stride_slot, k_stride_head;
+    void* v_pages;  int64_t v_pages_stride_page, v_pages_stride_slot, v_pages_stride_head;
+    const int32_t* block_table; int64_t table_stride, table_width;
+    const int32_t* seq_ids;                         /* [B*L] or NULL */
+    int64_t num_seqs, num_pages, page_size;
+} vtx_rotary_append_params;
+int vtx_rotary_append(const vtx_rotary_append_params* p, void* stream);
+
+/* vtx_paged_decode_attention: one new token of each of B sequences against its cache.  Query heads of q [B,Hq,D] share key
+ * heads in blocks of Hq/Hk; key j of sequence b lies at page block_table[b][j / page_size], slot j % page_size, of pools
+ * [num_pages, page_size, Hk, D] (element strides, unit stride over D).
+ *   out[b,h] = sum_j softmax_j(softmax_scale q[b,h] . k_j) v_j  over the last min(seqlens[b], window) keys (window 0: all)
+ *   lse[b,h] = log sum_j exp(softmax_scale q[b,h] . k_j), fp32 [B,Hq], or NULL
+ * seqlens int32 [B] are read on the device (capturable; the table may grow between replays); a sequence of no keys gives
+ * zeros and an lse of -inf.  block_table NULL: pools [B, page_size, Hk, D] of one page per sequence (a contiguous cache).
+ * Entries of the table behind a sequence's keys, or before its window, are not read.  Keys that the table gives no page, or
+ * that lie behind its width, are left out and set the device status word.
+ * fp32 accumulation; probabilities enter the second product as head and remainder of the I/O dtype.  D <= 256.
+ * scratch: vtx_paged_decode_scratch_bytes(p) bytes, 16-byte aligned, its contents of no meaning before and after the call
+ * (two calls that may overlap need two).  The reference calls flash_attn_with_kvcache (vortex/ops/attn_interface.py:1488). */
+typedef struct vtx_paged_decode_params {
+    const void* q;  int64_t q_stride_b, q_stride_h;
+    const void* k_pages; int64_t k_stride_page, k_stride_slot, k_stride_head;
+    const void* v_pages; int64_t v_stride_page, v_stride_slot, v_stride_head;
+    const int32_t* block_table; int64_t table_stride, table_width;   /* or NULL */
+    const int32_t* seqlens;
+    void* out;      int64_t out_stride_b, out_stride_h;
+    float* lse;
+    void* scratch;
+    double softmax_scale;
+    int64_t window;
+    int64_t B, Hq, Hk, D;
+    int64_t num_pages, page_size;
+    int64_t io_dtype;
+} vtx_paged_decode_params;
+int64_t vtx_paged_decode_scratch_bytes(const vtx_paged_decode_params* p);
+int vtx_paged_decode_attention(const vtx_paged_decode_params* p, void* stream);
+
+/* vtx_copy_pages: pool[dst[i]] = pool[src[i]] for i < pairs in each of `pools` pools of num_pages pages (page_bytes
+ * contiguous bytes each, page_stride_bytes apart).  src and dst are HOST arrays, read before the call returns and held by the
+ * launches themselves (a captured call replays the pages it was captured with).  A page may be copied to several; a dst that
+ * occurs twice, or that is also a src, is refused, as is an index outside the pool. */
+typedef struct vtx_copy_pages_params {
+    void* const* pool_ptrs;                         /* host array of device pointers */
+    const int64_t* src; const int64_t* dst;         /* host arrays */
+    int64_t pools, pairs, num_pages, page_bytes, page_stride_bytes;
+} vtx_copy_pages_params;
+int vtx_copy_pages(const vtx_copy_pages_params* p, void* stream);
 
 #ifdef __cplusplus
 }

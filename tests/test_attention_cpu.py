@@ -1,0 +1,146 @@
+"""CPU: what the attention-layer operators refuse before anything is launched, and the frequencies of rotated pairs."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from vortex_b200 import _lib, attn_ops
+
+
+def refused(fn, p, code, text):
+    assert fn(C.byref(p), None) == code and text in _lib.last_error(), _lib.last_error()
+
+
+def rotary(**kw):
+    base = dict(q=16, k=16, q_out=16, k_out=16, positions=16, inv_freq=16, rot=64, B=1, L=3, Hq=2, Hk=1, D=64, io_dtype=1, scale=1.0)
+    return _lib.RotaryParams(**{**base, **kw})
+
+
+@pytest.mark.parametrize("bad,code,text", [
+    (dict(io_dtype=7), -1, "dtype"), (dict(D=0), -1, "size"), (dict(L=-1), -1, "size"), (dict(D=513, rot=0), -2, "513"),
+    (dict(rot=65), -1, "rotated"), (dict(rot=66), -1, "rotated"), (dict(rot=-2), -1, "rotated"), (dict(q=None), -1, "null"),
+    (dict(k=None), -1, "null"), (dict(q_out=None), -1, "null"), (dict(positions=None), -1, "null"), (dict(inv_freq=None), -1, "null"),
+    (dict(q_weight=16, q_weight_dtype=9), -1, "weight"), (dict(Hq=1 << 20), -2, "heads")])
+def test_rotary_refusals(bad, code, text):
+    lib = _lib.lib()
+    refused(lib.vtx_qk_norm_rotary_fwd, rotary(**bad), code, text)
+    if "q_out" not in bad:
+        f = rotary(**bad)
+        refused(lib.vtx_qk_norm_rotary_bwd, _lib.RotaryBwdParams(fwd=f, dq_out=16, dk_out=16), code, text)
+        refused(lib.vtx_rotary_append, _lib.RotaryAppendParams(rot=f, v=16, k_pages=16, v_pages=16, block_table=16, table_width=2, num_seqs=3,
+                                                               num_pages=4, page_size=16), code, text)
+
+
+def test_rotary_of_nothing_needs_no_pointers():
+    for kw in (dict(L=0), dict(B=0), dict(Hq=0, Hk=0)):
+        p = rotary(q=None, k=None, q_out=None, k_out=None, **kw)
+        assert _lib.lib().vtx_qk_norm_rotary_fwd(C.byref(p), None) == 0
+
+
+def test_rotary_backward_refusals():
+    lib = _lib.lib()
+    f = rotary(q_weight=16, q_weight_dtype=0)
+    assert lib.vtx_qk_norm_rotary_bwd_scratch_bytes(C.byref(f)) % (2 * 64 * 4) == 0 < lib.vtx_qk_norm_rotary_bwd_scratch_bytes(C.byref(f))
+    assert lib.vtx_qk_norm_rotary_bwd_scratch_bytes(C.byref(rotary())) == 0
+    mk = lambda **kw: _lib.RotaryBwdParams(**{**dict(fwd=f, dq_out=16, dk_out=16, dq_weight=16, scratch=16), **kw})  # noqa: E731
+    refused(lib.vtx_qk_norm_rotary_bwd, mk(scratch=None), -1, "scratch")
+    refused(lib.vtx_qk_norm_rotary_bwd, mk(dq_weight=None), -1, "weight gradient")
+    refused(lib.vtx_qk_norm_rotary_bwd, mk(dk_out=None), -1, "null")
+    assert lib.vtx_qk_norm_rotary_bwd(None, None) == lib.vtx_qk_norm_rotary_fwd(None, None) == lib.vtx_rotary_append(None, None) == -1
+
+
+@pytest.mark.parametrize("bad,text", [(dict(page_size=0), "cache sizes"), (dict(num_pages=-1), "cache sizes"), (dict(v=None), "null"),
+                                      (dict(k_pages=None), "null"), (dict(block_table=None), "null"), (dict(num_seqs=2), "rows of the block table")])
+def test_append_refusals(bad, text):
+    base = dict(rot=rotary(), v=16, k_pages=16, v_pages=16, block_table=16, table_width=2, num_seqs=3, num_pages=4, page_size=16)
+    refused(_lib.lib().vtx_rotary_append, _lib.RotaryAppendParams(**{**base, **bad}), -1, text)
+    refused(_lib.lib().vtx_rotary_append, _lib.RotaryAppendParams(**{**base, "rot": rotary(Hk=0)}), -1, "key heads")
+
+
+def decode(**kw):
+    base = dict(q=16, k_pages=16, v_pages=16, block_table=16, table_width=8, seqlens=16, out=16, scratch=16, softmax_scale=1.0, B=2, Hq=8, Hk=2,
+                D=128, num_pages=40, page_size=16, io_dtype=1, q_stride_b=1024, q_stride_h=128, k_stride_page=4096, k_stride_slot=256,
+                k_stride_head=128, v_stride_page=4096, v_stride_slot=256, v_stride_head=128, out_stride_b=1024, out_stride_h=128)
+    return _lib.PagedDecodeParams(**{**base, **kw})
+
+
+@pytest.mark.parametrize("bad,code,text", [
+    (dict(io_dtype=3), -1, "dtype"), (dict(B=-1), -1, "sizes"), (dict(Hk=0), -1, "sizes"), (dict(Hq=7), -1, "7 query heads for 2"),
+    (dict(D=257), -2, "257"), (dict(D=0), -1, "sizes"), (dict(page_size=0), -1, "sizes"), (dict(window=-1), -1, "window"),
+    (dict(B=1 << 24), -2, "sequences"), (dict(num_pages=2 ** 31), -2, "pages"), (dict(block_table=None, num_pages=1), -1, "no block table"),
+    (dict(q=None), -1, "null"), (dict(k_pages=None), -1, "null"), (dict(seqlens=None), -1, "null"), (dict(out=None), -1, "null"),
+    (dict(scratch=None), -1, "scratch"), (dict(scratch=24), -1, "scratch")])
+def test_decode_attention_refusals(bad, code, text):
+    refused(_lib.lib().vtx_paged_decode_attention, decode(**bad), code, text)
+
+
+def test_decode_attention_scratch():
+    """Grows with the blocks that a call can use, not with its batch; nothing is needed where there is nothing to do."""
+    f = _lib.lib().vtx_paged_decode_scratch_bytes
+    n = lambda **kw: f(C.byref(decode(**kw)))  # noqa: E731
+    assert n(B=0) == 0 and n(Hq=7) == 0 and f(None) == 0
+    assert 0 < n(B=1, table_width=1) < n(B=1, table_width=100) < n(B=64, table_width=512) == n(B=4096, table_width=1 << 16)
+    assert n(B=64, table_width=512) < 8 << 20
+    assert n(B=64, table_width=2 ** 40, page_size=2 ** 30) > 0
+    assert all(n(B=b, table_width=w) % 8 == 0 for b in (1, 3) for w in (1, 7))
+    p = decode(B=0, q=None, k_pages=None, v_pages=None, out=None, scratch=None)
+    assert _lib.lib().vtx_paged_decode_attention(C.byref(p), None) == 0
+
+
+def copy(src_pages, dst_pages, **kw):
+    n = max(len(src_pages), 1)
+    a, b, ptrs = (C.c_int64 * n)(*src_pages), (C.c_int64 * n)(*dst_pages), (C.c_void_p * 2)(16, 32)
+    base = dict(pool_ptrs=C.cast(ptrs, C.c_void_p), src=C.cast(a, C.c_void_p), dst=C.cast(b, C.c_void_p), pools=2, pairs=len(src_pages), num_pages=10,
+                page_bytes=64, page_stride_bytes=64)
+    p = _lib.CopyPagesParams(**{**base, **kw})
+    return _lib.lib().vtx_copy_pages(C.byref(p), None), _lib.last_error()
+
+
+@pytest.mark.parametrize("src,dst,kw,text", [
+    ([0], [10], {}, "pool of 10"), ([-1], [1], {}, "pool of 10"), ([0, 1], [5, 5], {}, "page 5 is written twice"),
+    ([0, 1], [1, 2], {}, "both read and written"), ([3], [3], {}, "both read and written"), ([0], [1], dict(page_stride_bytes=63), "overlap"),
+    ([0], [1], dict(pools=-1), "negative"), ([0], [1], dict(pool_ptrs=None), "null"), ([0], [1], dict(src=None), "null")])
+def test_copy_pages_refusals(src, dst, kw, text):
+    rc, msg = copy(src, dst, **kw)
+    assert rc == -1 and text in msg
+
+
+def test_copy_pages_of_nothing():
+    assert copy([], [])[0] == 0 and copy([0], [1], pools=0)[0] == 0 and copy([0], [1], page_bytes=0, page_stride_bytes=0)[0] == 0
+    assert _lib.lib().vtx_copy_pages(None, None) == -1
+
+
+def test_cpu_tensors_are_rejected():
+    x, pos = torch.zeros(2, 4, 64), torch.arange(2)
+    fr, _ = attn_ops.rotary_inv_freq(64)
+    table = torch.zeros(2, 1, dtype=torch.int32)
+    pages = torch.zeros(2, 16, 4, 64)
+    for f in (lambda: attn_ops.qk_norm_rotary(x, x, pos, fr), lambda: attn_ops.rotary_append(x, x, x, pos, pages, pages, table, fr),
+              lambda: attn_ops.paged_decode_attention(x, pages, pages, table, table[:, 0]), lambda: attn_ops.copy_pages([pages], [0], [1])):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            f()
+    with pytest.raises(ValueError, match="2 sources for 1"):
+        attn_ops.copy_pages([pages], [0, 1], [1])
+
+
+def test_frequencies():
+    f, s = attn_ops.rotary_inv_freq(8, 10000.0)
+    assert f.dtype == torch.float64 and s == 1.0 and torch.allclose(f, torch.tensor([1, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-15)
+    f2, _ = attn_ops.rotary_inv_freq(8, scaling="linear", factor=128)
+    assert torch.equal(f2, f / 128)
+    f3, _ = attn_ops.rotary_inv_freq(8, scaling="ntk", factor=16.0)
+    assert f3[0] == 1 and abs(float(f3[-1] / f[-1]) - 1 / 16) < 1e-14
+    f4, s4 = attn_ops.rotary_inv_freq(128, scaling="yarn", factor=8.0, trained_length=4096)
+    f0, _ = attn_ops.rotary_inv_freq(128)
+    turns = 4096 * f0 / (2 * math.pi)
+    assert torch.equal(f4[turns > 32], f0[turns > 32]) and torch.equal(f4[turns < 1], f0[turns < 1] / 8)
+    mid = (turns > 1) & (turns < 32)
+    assert bool(((f4 < f0) & (f4 > f0 / 8))[mid].all()) and s4 == 0.1 * math.log(8) + 1
+    assert attn_ops.rotary_inv_freq(2)[0].tolist() == [1.0]
+    for kw in (dict(dim=7), dict(dim=0), dict(dim=8, factor=0), dict(dim=8, scaling="yarn"), dict(dim=2, scaling="ntk"),
+               dict(dim=8, scaling="yarn", trained_length=64, slow=2, fast=1)):
+        with pytest.raises(ValueError):
+            attn_ops.rotary_inv_freq(**kw)
+    with pytest.raises(NotImplementedError):
+        attn_ops.rotary_inv_freq(8, scaling="other")

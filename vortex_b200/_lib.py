@@ -16,7 +16,7 @@ QKV_SPLIT, QKV_INTERLEAVED, QKV_COLUMN_SPLIT = 0, 1, 2
 TAPS_XCORR, TAPS_CONV = 0, 1
 BIAS_NONE, BIAS_ADD, BIAS_GATED = 0, 1, 2
 
-_p, _i = C.c_void_p, C.c_int64
+_p, _i, _d = C.c_void_p, C.c_int64, C.c_double
 
 
 def header_abi_version() -> int:
@@ -31,11 +31,11 @@ def header_abi_version() -> int:
 
 
 def _struct(name, spec):
-    """spec: 'ptr:a i:b ...' -> ctypes.Structure subclass with 8-byte fields only."""
+    """spec: 'p:a i:b d:c ...' -> ctypes.Structure subclass with 8-byte fields only."""
     fields = []
     for item in spec.split():
         kind, fname = item.split(":")
-        fields.append((fname, _p if kind == "p" else _i))
+        fields.append((fname, {"p": _p, "i": _i, "d": _d}[kind]))
     return type(name, (C.Structure,), {"_fields_": fields})
 
 
@@ -127,9 +127,44 @@ class DecodeLayerParams(C.Structure):
                 ("io_dtype", _i)]
 
 
+RotaryParams = _struct("RotaryParams", """
+    p:q i:q_stride_b i:q_stride_l i:q_stride_h p:k i:k_stride_b i:k_stride_l i:k_stride_h
+    p:q_out i:q_out_stride_b i:q_out_stride_l i:q_out_stride_h p:k_out i:k_out_stride_b i:k_out_stride_l i:k_out_stride_h
+    p:positions i:positions_i64 i:pos_stride_b i:pos_stride_l p:inv_freq i:inv_freq_f64 i:rot
+    p:q_weight i:q_weight_dtype p:k_weight i:k_weight_dtype d:scale d:eps i:interleaved
+    i:B i:L i:Hq i:Hk i:D i:io_dtype""")
+
+
+class RotaryBwdParams(C.Structure):
+    _fields_ = [("fwd", RotaryParams),
+                ("dq_out", _p), ("dq_out_stride_b", _i), ("dq_out_stride_l", _i), ("dq_out_stride_h", _i),
+                ("dk_out", _p), ("dk_out_stride_b", _i), ("dk_out_stride_l", _i), ("dk_out_stride_h", _i),
+                ("dq_weight", _p), ("dk_weight", _p), ("scratch", _p)]
+
+
+class RotaryAppendParams(C.Structure):
+    _fields_ = [("rot", RotaryParams),
+                ("v", _p), ("v_stride_b", _i), ("v_stride_l", _i), ("v_stride_h", _i),
+                ("k_pages", _p), ("k_stride_page", _i), ("k_stride_slot", _i), ("k_stride_head", _i),
+                ("v_pages", _p), ("v_pages_stride_page", _i), ("v_pages_stride_slot", _i), ("v_pages_stride_head", _i),
+                ("block_table", _p), ("table_stride", _i), ("table_width", _i), ("seq_ids", _p),
+                ("num_seqs", _i), ("num_pages", _i), ("page_size", _i)]
+
+
+PagedDecodeParams = _struct("PagedDecodeParams", """
+    p:q i:q_stride_b i:q_stride_h p:k_pages i:k_stride_page i:k_stride_slot i:k_stride_head
+    p:v_pages i:v_stride_page i:v_stride_slot i:v_stride_head p:block_table i:table_stride i:table_width p:seqlens
+    p:out i:out_stride_b i:out_stride_h p:lse p:scratch d:softmax_scale i:window
+    i:B i:Hq i:Hk i:D i:num_pages i:page_size i:io_dtype""")
+
+CopyPagesParams = _struct("CopyPagesParams", """
+    p:pool_ptrs p:src p:dst i:pools i:pairs i:num_pages i:page_bytes i:page_stride_bytes""")
+
+
 STRUCTS = [FeaturizerParams, GcgParams, FusedFirParams, ModalParams, IirParams, StepFirParams, StepIirParams,
            DecodeLayerParams, FusedIirParams, HyenaXParams, CausalConv1dParams, CausalConv1dUpdateParams,
-           VarlenStatesParams, GcgClParams, GcgBwdParams]
+           VarlenStatesParams, GcgClParams, GcgBwdParams, RotaryParams, RotaryBwdParams, RotaryAppendParams,
+           PagedDecodeParams, CopyPagesParams]
 
 # name -> (restype, argtypes); every symbol include/vortex_b200.h declares
 SYMBOLS = {
@@ -160,6 +195,13 @@ SYMBOLS = {
     "vtx_step_fir": (C.c_int, [C.POINTER(StepFirParams), _p]),
     "vtx_step_iir": (C.c_int, [C.POINTER(StepIirParams), _p]),
     "vtx_decode_layer": (C.c_int, [C.POINTER(DecodeLayerParams), _p]),
+    "vtx_qk_norm_rotary_fwd": (C.c_int, [C.POINTER(RotaryParams), _p]),
+    "vtx_qk_norm_rotary_bwd_scratch_bytes": (_i, [C.POINTER(RotaryParams)]),
+    "vtx_qk_norm_rotary_bwd": (C.c_int, [C.POINTER(RotaryBwdParams), _p]),
+    "vtx_rotary_append": (C.c_int, [C.POINTER(RotaryAppendParams), _p]),
+    "vtx_paged_decode_scratch_bytes": (_i, [C.POINTER(PagedDecodeParams)]),
+    "vtx_paged_decode_attention": (C.c_int, [C.POINTER(PagedDecodeParams), _p]),
+    "vtx_copy_pages": (C.c_int, [C.POINTER(CopyPagesParams), _p]),
 }
 
 _host = None
@@ -208,8 +250,7 @@ def host():
         if mod.abi_version() != header_abi_version():
             raise RuntimeError(f"{HOST_PATH} was built for ABI version {mod.abi_version()}: rebuild it with "
                                "`python -m vortex_b200.build`")
-        mod.bind(*(C.cast(getattr(handle, n), _p).value for n in
-                   ("vtx_decode_layer", "vtx_fused_fir_fwd", "vtx_fused_iir_fwd", "vtx_fused_iir_scratch_bytes", "vtx_last_error")))
+        mod.bind({n: C.cast(getattr(handle, n), _p).value for n in SYMBOLS})
         _host = mod
     return _host
 

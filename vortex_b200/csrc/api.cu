@@ -2,6 +2,7 @@
 #include <atomic>
 #include <cstring>
 
+#include "attn.cuh"
 #include "common.cuh"
 #include "tma.cuh"
 
@@ -113,7 +114,10 @@ extern "C" int vtx_device_status(void) {
         int v = r->take();
         if (v && !worst) worst = v;
     }
-    if (worst) vtx::fail(VTX_ERR_DEVICE, "a kernel gave up a bounded wait (code %d)", worst);
+    if (worst == vtx::kStatusBadPage)
+        vtx::fail(VTX_ERR_DEVICE, "a block table gave no page for a token that a call had to store or read");
+    else if (worst)
+        vtx::fail(VTX_ERR_DEVICE, "a kernel gave up a bounded wait (code %d)", worst);
     return worst ? VTX_ERR_DEVICE : VTX_OK;
 }
 
@@ -154,6 +158,11 @@ extern "C" int64_t vtx_struct_size(int64_t which) {
         case 12: return sizeof(vtx_varlen_states_params);
         case 13: return sizeof(vtx_gcg_cl_params);
         case 14: return sizeof(vtx_gcg_bwd_params);
+        case 15: return sizeof(vtx_rotary_params);
+        case 16: return sizeof(vtx_rotary_bwd_params);
+        case 17: return sizeof(vtx_rotary_append_params);
+        case 18: return sizeof(vtx_paged_decode_params);
+        case 19: return sizeof(vtx_copy_pages_params);
         default: return -1;
     }
 }

@@ -8,6 +8,9 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/types.h>
 
+#include <cmath>
+#include <map>
+
 #include "../../include/vortex_b200.h"
 
 namespace py = pybind11;
@@ -21,6 +24,13 @@ decltype(&vtx_fused_fir_fwd) p_fused_fir_fwd;
 decltype(&vtx_fused_iir_fwd) p_fused_iir_fwd;
 decltype(&vtx_fused_iir_scratch_bytes) p_fused_iir_scratch_bytes;
 decltype(&vtx_last_error) p_last_error;
+decltype(&vtx_qk_norm_rotary_fwd) p_rotary_fwd;
+decltype(&vtx_qk_norm_rotary_bwd) p_rotary_bwd;
+decltype(&vtx_qk_norm_rotary_bwd_scratch_bytes) p_rotary_bwd_scratch_bytes;
+decltype(&vtx_rotary_append) p_rotary_append;
+decltype(&vtx_paged_decode_attention) p_paged_decode;
+decltype(&vtx_paged_decode_scratch_bytes) p_paged_decode_scratch_bytes;
+decltype(&vtx_copy_pages) p_copy_pages;
 
 // The entry points run without the GIL (see the module definition); an error is made with it.
 [[noreturn]] void raise(PyObject* type, const std::string& msg) {
@@ -244,20 +254,272 @@ std::tuple<Tensor, Opt> fused_iir_fwd(Tensor u, const Tensor& w3_, const Tensor&
     return {y, st};
 }
 
+// ---- attention layers ----------------------------------------------------------------------------------------------------
+[[noreturn]] void bad(const std::string& msg) { raise(PyExc_ValueError, msg); }
+void same_device(const Tensor& t, const Tensor& like) {
+    need_cuda(t);
+    if (t.device() != like.device()) raise(PyExc_RuntimeError, "vortex_b200: tensors on different devices");
+}
+// [B, L, H, D] view of [T, H, D] or [B, L, H, D] rows, unit stride over D
+struct Rows4 {
+    Tensor t;
+    int64_t B, L, H, D, sb, sl, sh;
+    Rows4(const Tensor& x, const char* name) : t(x) {
+        if (t.dim() != 3 && t.dim() != 4) bad(std::string(name) + " must be [T, H, D] or [B, L, H, D], got " + str(t));
+        if (t.size(-1) != 1 && t.stride(-1) != 1) t = t.contiguous();
+        const bool four = t.dim() == 4;
+        B = four ? t.size(0) : 1; L = t.size(four ? 1 : 0); H = t.size(-2); D = t.size(-1);
+        sb = four ? t.stride(0) : 0; sl = t.stride(four ? 1 : 0); sh = t.stride(-2);
+    }
+    bool tokens_as(const Rows4& o) const { return t.dim() == o.t.dim() && B == o.B && L == o.L && D == o.D; }
+};
+
+struct Rotary {
+    vtx_rotary_params p{};
+    std::vector<Tensor> keep;
+    Rotary(const Rows4& q, const Rows4* k, const Opt& positions_, const Opt& inv_freq_, const Opt& qw, const Opt& kw, double eps, bool interleaved, double scale) {
+        p.io_dtype = code(q.t);
+        p.B = q.B; p.L = q.L; p.D = q.D; p.Hq = q.H;
+        p.q = ptr(q.t); p.q_stride_b = q.sb; p.q_stride_l = q.sl; p.q_stride_h = q.sh;
+        if (k) {
+            same_device(k->t, q.t);
+            if (!k->tokens_as(q) || k->t.scalar_type() != q.t.scalar_type())
+                bad("k must have the tokens, head size and dtype of q: " + str(k->t) + " beside " + str(q.t));
+            p.Hk = k->H;
+            p.k = ptr(k->t); p.k_stride_b = k->sb; p.k_stride_l = k->sl; p.k_stride_h = k->sh;
+        }
+        if (positions_) {
+            Tensor pos = *positions_;
+            same_device(pos, q.t);
+            if (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) raise(PyExc_TypeError, "positions must be int32 or int64");
+            p.positions_i64 = pos.scalar_type() == at::kLong;
+            if (q.t.dim() == 4 && pos.dim() == 2 && pos.size(0) == q.B && pos.size(1) == q.L) {
+                p.pos_stride_b = pos.stride(0); p.pos_stride_l = pos.stride(1);
+            } else if (pos.dim() == 1 && pos.size(0) == q.L) {          // [T], or [L] for every batch element
+                p.pos_stride_l = pos.stride(0);
+            } else {
+                bad("positions have shape " + str(pos) + " for tokens of " + str(q.t));
+            }
+            p.positions = ptr(pos);
+            keep.push_back(pos);
+        }
+        if (inv_freq_) {
+            Tensor f = *inv_freq_;
+            same_device(f, q.t);
+            if (f.scalar_type() != at::kDouble && f.scalar_type() != at::kFloat) raise(PyExc_TypeError, "inv_freq must be float64 or float32");
+            if (f.dim() != 1 || 2 * f.size(0) > q.D) bad("inv_freq must be [rot / 2] with rot <= " + std::to_string(q.D) + ", got " + str(f));
+            f = f.contiguous();
+            p.inv_freq = ptr(f); p.inv_freq_f64 = f.scalar_type() == at::kDouble; p.rot = 2 * f.size(0);
+            keep.push_back(f);
+        }
+        auto weight = [&](const Opt& w, const char* name, const void*& at, int64_t& dt) {
+            if (!w) return;
+            need_cuda(*w);
+            Tensor t = param(*w, q.t);
+            if (t.dim() != 1 || t.size(0) != q.D) bad(std::string(name) + " must be [" + std::to_string(q.D) + "], got " + str(t));
+            at = ptr(t); dt = code(t);
+            keep.push_back(t);
+        };
+        weight(qw, "q_weight", p.q_weight, p.q_weight_dtype);
+        weight(kw, "k_weight", p.k_weight, p.k_weight_dtype);
+        p.eps = eps; p.interleaved = interleaved; p.scale = scale;
+    }
+    void q_to(const Tensor& t) { const Rows4 r(t, "q"); p.q_out = out(t); p.q_out_stride_b = r.sb; p.q_out_stride_l = r.sl; p.q_out_stride_h = r.sh; }
+    void k_to(const Tensor& t) { const Rows4 r(t, "k"); p.k_out = out(t); p.k_out_stride_b = r.sb; p.k_out_stride_l = r.sl; p.k_out_stride_h = r.sh; }
+};
+
+std::tuple<Tensor, Opt> qk_norm_rotary(const Tensor& q_, const Opt& k_, const Tensor& positions, const Tensor& inv_freq, const Opt& qw, const Opt& kw,
+                                       double eps, bool interleaved, double scale) {
+    need_cuda(q_);
+    const Rows4 q(q_, "q");
+    std::optional<Rows4> k;
+    if (k_) { need_cuda(*k_); k.emplace(*k_, "k"); }
+    else if (kw) bad("k_weight without k");
+    Rotary r(q, k ? &*k : nullptr, positions, inv_freq, qw, kw, eps, interleaved, scale);
+    Tensor qo = empty(q.t.sizes(), q.t, q.t.scalar_type());
+    Opt ko;
+    r.q_to(qo);
+    if (k) { ko = empty(k->t.sizes(), q.t, q.t.scalar_type()); r.k_to(*ko); }
+    const c10::cuda::CUDAGuard on(q.t.device());
+    check(p_rotary_fwd(&r.p, stream_of(q.t)));
+    return {qo, ko};
+}
+
+std::tuple<Tensor, Opt, Opt, Opt> qk_norm_rotary_bwd(const Tensor& dq_, const Opt& dk_, const Tensor& q_, const Opt& k_, const Tensor& positions,
+                                                     const Tensor& inv_freq, const Opt& qw, const Opt& kw, double eps, bool interleaved, double scale) {
+    need_cuda(q_);
+    const Rows4 q(q_, "q"), dq(dq_, "dq");
+    std::optional<Rows4> k, dk;
+    if (k_) {
+        need_cuda(*k_);
+        k.emplace(*k_, "k");
+        dk.emplace(have(dk_, "shape"), "dk");
+    }
+    Rotary r(q, k ? &*k : nullptr, positions, inv_freq, qw, kw, eps, interleaved, scale);
+    vtx_rotary_bwd_params p{};
+    auto grad = [&](const Rows4& d, const Rows4& x, const void*& at, int64_t& sb, int64_t& sl, int64_t& sh) {
+        same_device(d.t, q.t);
+        if (d.t.sizes() != x.t.sizes() || d.t.scalar_type() != x.t.scalar_type()) bad("a gradient has shape " + str(d.t) + " or dtype other than its tensor's");
+        at = ptr(d.t); sb = d.sb; sl = d.sl; sh = d.sh;
+    };
+    grad(dq, q, p.dq_out, p.dq_out_stride_b, p.dq_out_stride_l, p.dq_out_stride_h);
+    if (k) grad(*dk, *k, p.dk_out, p.dk_out_stride_b, p.dk_out_stride_l, p.dk_out_stride_h);
+    Tensor gq = empty(q.t.sizes(), q.t, q.t.scalar_type()), scratch;
+    Opt gk, gqw, gkw;
+    r.q_to(gq);
+    if (k) { gk = empty(k->t.sizes(), q.t, q.t.scalar_type()); r.k_to(*gk); }
+    auto dtype_of = [](int64_t c) { return c == VTX_F32 ? at::kFloat : c == VTX_BF16 ? at::kBFloat16 : at::kHalf; };
+    if (qw) { gqw = empty({q.D}, q.t, dtype_of(r.p.q_weight_dtype)); p.dq_weight = out(*gqw); }
+    if (kw) { gkw = empty({q.D}, q.t, dtype_of(r.p.k_weight_dtype)); p.dk_weight = out(*gkw); }
+    p.fwd = r.p;
+    const int64_t need = p_rotary_bwd_scratch_bytes(&p.fwd);
+    if (need > 0) { scratch = empty({need}, q.t, at::kByte); p.scratch = out(scratch); }
+    const c10::cuda::CUDAGuard on(q.t.device());
+    check(p_rotary_bwd(&p, stream_of(q.t)));
+    return {gq, gk, gqw, gkw};
+}
+
+struct Pool {
+    int64_t pages, size, sp, ss, sh;
+    Pool(const Tensor& t, const char* name, const Tensor& like, int64_t Hk, int64_t D) {
+        same_device(t, like);
+        if (t.dim() != 4 || t.size(2) != Hk || t.size(3) != D || t.scalar_type() != like.scalar_type())
+            bad(std::string(name) + " must be [pages, page_size, " + std::to_string(Hk) + ", " + std::to_string(D) + "] of q's dtype, got " + str(t));
+        if (D != 1 && t.stride(3) != 1) bad(std::string(name) + " must have unit stride over the head's values");
+        pages = t.size(0); size = t.size(1); sp = t.stride(0); ss = t.stride(1); sh = t.stride(2);
+    }
+};
+void int32_on(const Tensor& t, const char* name, const Tensor& like, int64_t dims) {
+    same_device(t, like);
+    if (t.scalar_type() != at::kInt) raise(PyExc_TypeError, std::string(name) + " must be int32");
+    if (t.dim() != dims || (t.size(-1) > 1 && t.stride(-1) != 1)) bad(std::string(name) + " must be a dense " + std::to_string(dims) + "-dimensional tensor, got " + str(t));
+}
+
+Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& positions, const Tensor& k_pages, const Tensor& v_pages,
+                     const Tensor& table, const Opt& inv_freq, const Opt& qw, const Opt& kw, const Opt& seq_ids, double eps, bool interleaved,
+                     double scale) {
+    need_cuda(q_); need_cuda(k_); need_cuda(v_);
+    const Rows4 q(q_, "q"), k(k_, "k"), v(v_, "v");
+    Rotary r(q, &k, positions, inv_freq, qw, kw, eps, interleaved, scale);
+    same_device(v.t, q.t);
+    if (v.t.sizes() != k.t.sizes() || v.t.scalar_type() != k.t.scalar_type()) bad("v must have the shape and dtype of k");
+    const Pool kp(k_pages, "k_pages", q.t, k.H, k.D), vp(v_pages, "v_pages", q.t, k.H, k.D);
+    if (kp.pages != vp.pages || kp.size != vp.size || kp.size < 1) bad("k_pages and v_pages must have the same pages, of at least one token");
+    for (const Tensor* t : {&k_pages, &v_pages})
+        for (int i = 0; i < 4; ++i)
+            if (t->size(i) > 1 && t->stride(i) == 0) bad("the pools are written: no dimension of theirs may be expanded");
+    int32_on(table, "block_table", q.t, 2);
+    vtx_rotary_append_params p{};
+    Tensor qo = empty(q.t.sizes(), q.t, q.t.scalar_type());
+    r.q_to(qo);
+    p.rot = r.p;
+    p.v = ptr(v.t); p.v_stride_b = v.sb; p.v_stride_l = v.sl; p.v_stride_h = v.sh;
+    p.k_pages = out(k_pages); p.k_stride_page = kp.sp; p.k_stride_slot = kp.ss; p.k_stride_head = kp.sh;
+    p.v_pages = out(v_pages); p.v_pages_stride_page = vp.sp; p.v_pages_stride_slot = vp.ss; p.v_pages_stride_head = vp.sh;
+    p.block_table = static_cast<const int32_t*>(ptr(table)); p.table_stride = table.stride(0); p.table_width = table.size(1);
+    p.num_seqs = table.size(0); p.num_pages = kp.pages; p.page_size = kp.size;
+    if (seq_ids) {
+        int32_on(*seq_ids, "seq_ids", q.t, 1);
+        if (seq_ids->size(0) != q.B * q.L) bad("seq_ids must name a row of the block table for each of the " + std::to_string(q.B * q.L) + " tokens");
+        p.seq_ids = static_cast<const int32_t*>(ptr(*seq_ids));
+    } else if (q.B * q.L != p.num_seqs) {
+        bad("without seq_ids there is one token for every row of the block table: " + std::to_string(q.B * q.L) + " tokens, " +
+            std::to_string(p.num_seqs) + " rows");
+    }
+    const c10::cuda::CUDAGuard on(q.t.device());
+    check(p_rotary_append(&p, stream_of(q.t)));
+    return qo;
+}
+
+std::tuple<Tensor, Opt> paged_decode_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages, const Opt& table, const Tensor& seqlens,
+                                               std::optional<double> softmax_scale, int64_t window, bool want_lse) {
+    need_cuda(q_);
+    if (q_.dim() != 3) bad("q must be [B, H, D], got " + str(q_));
+    const Tensor q = q_.size(2) != 1 && q_.stride(2) != 1 ? q_.contiguous() : q_;
+    if (k_pages.dim() != 4) bad("k_pages must be [pages, page_size, H, D], got " + str(k_pages));
+    vtx_paged_decode_params p{};
+    p.io_dtype = code(q);
+    p.B = q.size(0); p.Hq = q.size(1); p.D = q.size(2); p.Hk = k_pages.size(2);
+    const Pool kp(k_pages, "k_pages", q, p.Hk, p.D), vp(v_pages, "v_pages", q, p.Hk, p.D);
+    if (kp.pages != vp.pages || kp.size != vp.size) bad("k_pages and v_pages must have the same pages");
+    int32_on(seqlens, "seqlens", q, 1);
+    if (seqlens.size(0) != p.B) bad("seqlens must be [" + std::to_string(p.B) + "], got " + str(seqlens));
+    if (table) {
+        int32_on(*table, "block_table", q, 2);
+        if (table->size(0) != p.B || table->size(1) < 1) bad("block_table must be [" + std::to_string(p.B) + ", pages of a sequence], got " + str(*table));
+        p.block_table = static_cast<const int32_t*>(ptr(*table)); p.table_stride = table->stride(0); p.table_width = table->size(1);
+    } else if (kp.pages != p.B) {
+        bad("without a block_table the caches must be [B, keys, H, D]");
+    }
+    Tensor o = empty(q.sizes(), q, q.scalar_type()), scratch;
+    Opt lse;
+    if (want_lse) { lse = empty({p.B, p.Hq}, q, at::kFloat); p.lse = static_cast<float*>(out(*lse)); }
+    p.q = ptr(q); p.q_stride_b = q.stride(0); p.q_stride_h = q.stride(1);
+    p.k_pages = ptr(k_pages); p.k_stride_page = kp.sp; p.k_stride_slot = kp.ss; p.k_stride_head = kp.sh;
+    p.v_pages = ptr(v_pages); p.v_stride_page = vp.sp; p.v_stride_slot = vp.ss; p.v_stride_head = vp.sh;
+    p.seqlens = static_cast<const int32_t*>(ptr(seqlens));
+    p.out = out(o); p.out_stride_b = o.stride(0); p.out_stride_h = o.stride(1);
+    p.softmax_scale = softmax_scale ? *softmax_scale : 1.0 / std::sqrt((double)p.D);
+    p.window = window; p.num_pages = kp.pages; p.page_size = kp.size;
+    const c10::cuda::CUDAGuard on(q.device());
+    const int64_t need = p_paged_decode_scratch_bytes(&p);
+    if (need > 0) { scratch = empty({need}, q, at::kByte); p.scratch = out(scratch); }
+    check(p_paged_decode(&p, stream_of(q)));
+    return {o, lse};
+}
+
+void copy_pages(const std::vector<Tensor>& pools, const std::vector<int64_t>& src, const std::vector<int64_t>& dst) {
+    if (src.size() != dst.size()) bad("copy_pages: " + std::to_string(src.size()) + " sources for " + std::to_string(dst.size()) + " destinations");
+    if (pools.empty()) return;
+    vtx_copy_pages_params p{};
+    const Tensor& first = pools[0];
+    std::vector<void*> at;
+    for (const Tensor& t : pools) {
+        same_device(t, first);
+        if (t.dim() < 1 || t.sizes() != first.sizes() || t.strides() != first.strides() || t.scalar_type() != first.scalar_type())
+            bad("copy_pages: the pools must have one shape, layout and dtype");
+        at.push_back(out(t));
+    }
+    const int64_t n = first.size(0), es = first.element_size();
+    int64_t page = 1;
+    for (int64_t i = first.dim() - 1; i > 0; --i) {
+        if (first.size(i) > 1 && first.stride(i) != page) bad("copy_pages: a page must be contiguous");
+        page *= first.size(i);
+    }
+    p.pool_ptrs = at.data(); p.src = src.data(); p.dst = dst.data();
+    p.pools = (int64_t)pools.size(); p.pairs = (int64_t)src.size(); p.num_pages = n;
+    p.page_bytes = page * es; p.page_stride_bytes = n > 1 ? first.stride(0) * es : page * es;
+    const c10::cuda::CUDAGuard on(first.device());
+    check(p_copy_pages(&p, stream_of(first)));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_vtx_host, m) {
     m.def("abi_version", [] { return VTX_ABI_VERSION; });
-    m.def("bind", [](uintptr_t decode, uintptr_t fir, uintptr_t iir, uintptr_t iir_scratch, uintptr_t last_error) {
-        p_decode_layer = reinterpret_cast<decltype(p_decode_layer)>(decode);
-        p_fused_fir_fwd = reinterpret_cast<decltype(p_fused_fir_fwd)>(fir);
-        p_fused_iir_fwd = reinterpret_cast<decltype(p_fused_iir_fwd)>(iir);
-        p_fused_iir_scratch_bytes = reinterpret_cast<decltype(p_fused_iir_scratch_bytes)>(iir_scratch);
-        p_last_error = reinterpret_cast<decltype(p_last_error)>(last_error);
+    // addresses of the library's functions by name; all that this module calls must be among them
+    m.def("bind", [](const std::map<std::string, uintptr_t>& f) {
+        p_decode_layer = reinterpret_cast<decltype(p_decode_layer)>(f.at("vtx_decode_layer"));
+        p_fused_fir_fwd = reinterpret_cast<decltype(p_fused_fir_fwd)>(f.at("vtx_fused_fir_fwd"));
+        p_fused_iir_fwd = reinterpret_cast<decltype(p_fused_iir_fwd)>(f.at("vtx_fused_iir_fwd"));
+        p_fused_iir_scratch_bytes = reinterpret_cast<decltype(p_fused_iir_scratch_bytes)>(f.at("vtx_fused_iir_scratch_bytes"));
+        p_last_error = reinterpret_cast<decltype(p_last_error)>(f.at("vtx_last_error"));
+        p_rotary_fwd = reinterpret_cast<decltype(p_rotary_fwd)>(f.at("vtx_qk_norm_rotary_fwd"));
+        p_rotary_bwd = reinterpret_cast<decltype(p_rotary_bwd)>(f.at("vtx_qk_norm_rotary_bwd"));
+        p_rotary_bwd_scratch_bytes = reinterpret_cast<decltype(p_rotary_bwd_scratch_bytes)>(f.at("vtx_qk_norm_rotary_bwd_scratch_bytes"));
+        p_rotary_append = reinterpret_cast<decltype(p_rotary_append)>(f.at("vtx_rotary_append"));
+        p_paged_decode = reinterpret_cast<decltype(p_paged_decode)>(f.at("vtx_paged_decode_attention"));
+        p_paged_decode_scratch_bytes = reinterpret_cast<decltype(p_paged_decode_scratch_bytes)>(f.at("vtx_paged_decode_scratch_bytes"));
+        p_copy_pages = reinterpret_cast<decltype(p_copy_pages)>(f.at("vtx_copy_pages"));
     });
     // Without the GIL, as torch's own calls and calls through ctypes are: an allocation or a launch into a full queue can
     // block, and the process's other threads go on meanwhile.
     m.def("decode_layer", &decode_layer, py::call_guard<py::gil_scoped_release>());
     m.def("fused_fir_fwd", &fused_fir_fwd, py::call_guard<py::gil_scoped_release>());
     m.def("fused_iir_fwd", &fused_iir_fwd, py::call_guard<py::gil_scoped_release>());
+    m.def("qk_norm_rotary", &qk_norm_rotary, py::call_guard<py::gil_scoped_release>());
+    m.def("qk_norm_rotary_bwd", &qk_norm_rotary_bwd, py::call_guard<py::gil_scoped_release>());
+    m.def("rotary_append", &rotary_append, py::call_guard<py::gil_scoped_release>());
+    m.def("paged_decode_attention", &paged_decode_attention, py::call_guard<py::gil_scoped_release>());
+    m.def("copy_pages", &copy_pages, py::call_guard<py::gil_scoped_release>());
 }

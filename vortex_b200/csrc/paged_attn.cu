@@ -1,0 +1,843 @@
+// Attention of one new token per sequence over a cache of keys and values in pages.
+//
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp2(s_j - m),  s_j = log2(e) * softmax_scale * (q . k_j)
+//
+// in one pass over the cache with a running maximum m.  Every key and value is read once for up to 16 query heads, two
+// operations a byte and head: memory bounds it.  What the kernels are built around:
+//
+// * Work.  The cache is cut into units of 64 keys of one key head; the units of all sequences and heads, in a row, are dealt
+//   out to the blocks in equal runs, whatever the lengths (they are on the device: every block sums them up itself).  A run
+//   covers the end of one (sequence, head), some whole ones, and the beginning of another; whole ones are finished in place,
+//   the two open ones leave (m, sum, unnormalised out) in the scratch, which the second kernel joins.  At most two open ones a
+//   block: the scratch does not grow with the batch.  Launched so that it is set up while the first kernel still runs.
+// * No shared memory on the way.  With keys as the rows of the first product (S^T = K Q^T) a lane's piece of the A operand is
+//   16 contiguous bytes of two key rows, once the order of the summed dimensions is agreed with Q; for the second
+//   (O^T = V^T P^T) it is 16 contiguous bytes of four value rows, after one byte permutation a register.  So loads go from
+//   global memory to the registers that the mma.sync reads; 16 keys are 16 loads of 16 bytes a lane, the next tile's keys are
+//   in flight from the moment the scores exist, its values from the moment the second product is issued.  Tensor cores at
+//   16 x 8 x 16 are enough: even with one query head of eight columns they are under a tenth busy.
+// * P is brought from the accumulator's layout to the B operand's by transposing 8 x 8 blocks (movmatrix), as head and
+//   remainder: rounded to bf16 alone it would cost as much as the output's own rounding.
+// * The maximum is raised only when a score passes it by more than a slack (2^8, for fp16 2^4): most tiles then need neither
+//   the reduction over the lanes nor the rescaling; the sums stay below 2^15 * keys, far inside fp32.
+#include <cfloat>
+
+#include "attn.cuh"
+#include "tma.cuh"
+
+VTX_DEFINE_STATUS_READER()
+
+namespace vtx {
+namespace {
+
+constexpr int kThreads = 128, kWarps = 4, kTile = 16, kUnit = kWarps * kTile;
+// Reference m of a running sum: p = exp2(s - m).  The largest score seen stays between m + shift and m + shift + slack.
+// fp16 keeps nothing below 2^-25: its probabilities are held near the top of its range (at most 2^15), so that even 2^20 keys
+// of 2^-25 of the largest one's weight still count; bf16 and fp32 need no shift.
+template <typename T> struct Ref { static constexpr float shift = 0.f, slack = 8.f; };
+template <> struct Ref<__half> { static constexpr float shift = 11.f, slack = 4.f; };
+
+struct AttnArgs {
+    const void* q;
+    int64_t qsb, qsh;
+    const void* k;
+    int64_t ksp, kss, ksh;
+    const void* v;
+    int64_t vsp, vss, vsh;
+    const int32_t* table;           // NULL: page b is sequence b's
+    int64_t ts;
+    const int32_t* lens;
+    void* out;
+    int64_t osb, osh;
+    float* lse;
+    float* part;                    // [blocks][2][heads of a pass] rows of (DP sums)
+    float2* part_ml;                // the same, (m, l)
+    struct Open* open;              // [blocks]
+    float scale;                    // log2(e) * softmax_scale
+    int window;                     // INT_MAX: none
+    int B, Hq, G, D, page_size, num_pages;
+    int passes, head_groups;        // passes over the G query heads of a key head; Hk * passes
+    int64_t max_keys;
+};
+
+// The (sequence, head group) that begins in a block's run and ends in the run of block `last`.
+struct Open {
+    int64_t units;                  // of the whole call
+    int b, hg, last, pad;
+};
+
+struct Seq {                        // keys lo .. n-1 of a sequence; tiles start at lo & ~15
+    int lo, n, base, units;
+    __device__ Seq(const AttnArgs& a, int b) {
+        const int len = a.lens[b];
+        n = len < 0 ? 0 : len;
+        if (n > a.max_keys) {
+            atomicCAS(&g_device_status, 0, kStatusBadPage);
+            n = (int)a.max_keys;
+        }
+        lo = (len > a.window) ? len - a.window : 0;
+        if (lo > n) lo = n;
+        base = lo & ~(kTile - 1);
+        units = n > base ? (n - base + kUnit - 1) / kUnit : 1;      // an empty one has a unit, to write its zeros
+    }
+};
+
+__device__ __forceinline__ int64_t run_start(int64_t units, int w, int W) { return units * w / W; }
+
+__device__ __forceinline__ int64_t warp_scan(int64_t v) {
+    const int lane = threadIdx.x & 31;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+// Inclusive sum over the block's threads, and the block's total.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_tot, int64_t& total) {
+    v = warp_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 31) s_tot[threadIdx.x >> 5] = v;
+    __syncthreads();
+    total = 0;
+    int64_t before = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < (int)(threadIdx.x >> 5)) before += s_tot[w];
+        total += s_tot[w];
+    }
+    return v + before;
+}
+
+// The block's run of units and the sequence in which it starts.
+struct Run {
+    int64_t units, at, end, seq_first;     // of all; next, end; first unit of sequence b
+    int b;
+    __device__ Run(const AttnArgs& a) {
+        __shared__ int64_t s_tot[kWarps], s_first;
+        __shared__ int s_b;
+        const int tid = threadIdx.x;
+        int64_t mine = tid < a.B ? (int64_t)Seq(a, tid).units * a.head_groups : 0, total, incl;
+        incl = block_scan(mine, s_tot, total);
+        units = total;
+        for (int c = kThreads; c < a.B; c += kThreads) {
+            int64_t t;
+            block_scan(c + tid < a.B ? (int64_t)Seq(a, c + tid).units * a.head_groups : 0, s_tot, t);
+            units += t;
+        }
+        at = run_start(units, blockIdx.x, gridDim.x);
+        end = run_start(units, blockIdx.x + 1, gridDim.x);
+        int64_t before = 0;
+        for (int c = 0;; c += kThreads) {
+            if (c) {
+                mine = c + tid < a.B ? (int64_t)Seq(a, c + tid).units * a.head_groups : 0;
+                incl = block_scan(mine, s_tot, total);
+            }
+            if (at < before + total || c + kThreads >= a.B) {
+                const int64_t first = before + incl - mine;
+                if (at >= first && at < first + mine) { s_b = c + tid; s_first = first; }
+                break;
+            }
+            before += total;
+        }
+        __syncthreads();
+        b = s_b;
+        seq_first = s_first;
+    }
+};
+
+// One piece of work: units c0 .. c1-1 of a sequence and head group.
+struct Piece {
+    int b, hg, c0, c1, units, lo, n, base;
+    int kvh, h0, heads;                    // key head, first query head, query heads
+};
+
+template <int HP> __device__ __forceinline__ Piece next_piece(const AttnArgs& a, Run& r) {
+    const Seq s(a, r.b);
+    Piece p;
+    p.b = r.b; p.units = s.units; p.lo = s.lo; p.n = s.n; p.base = s.base;
+    const int64_t in = r.at - r.seq_first;
+    p.hg = (int)(in / s.units);
+    p.c0 = (int)(in - (int64_t)p.hg * s.units);
+    const int64_t left = r.end - r.at;
+    p.c1 = (int)(p.c0 + left < s.units ? p.c0 + left : s.units);
+    p.kvh = p.hg / a.passes;
+    const int first = (p.hg - p.kvh * a.passes) * HP;
+    p.h0 = p.kvh * a.G + first;
+    p.heads = a.G - first < HP ? a.G - first : HP;
+    r.at += p.c1 - p.c0;
+    if (p.hg == a.head_groups - 1 && p.c1 == s.units) {
+        r.seq_first += (int64_t)s.units * a.head_groups;
+        ++r.b;
+    }
+    return p;
+}
+
+// The warps' (m, l, out) of a piece, in shared memory, joined: a whole (sequence, head group) is finished, an open one stored.
+template <typename T, int DP, int HP, int PITCH>
+__device__ __forceinline__ void join_warps(const AttnArgs& a, const Piece& p, const Run& r, const float* s_o, const float (*s_m)[HP],
+                                           const float (*s_l)[HP], bool vec) {
+    const bool whole = p.c0 == 0 && p.c1 == p.units;
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (p.c0 == 0);
+    for (int i = threadIdx.x; i < p.heads * (DP / 4); i += kThreads) {
+        const int h = i / (DP / 4), d = (i - h * (DP / 4)) * 4;
+        float m = s_m[0][h];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w][h]);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = exp2f(s_m[w][h] - m);
+            const float4 x = *reinterpret_cast<const float4*>(s_o + (w * HP + h) * PITCH + d);
+            o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+            l += f * s_l[w][h];
+        }
+        if (whole) {
+            // (no key at all: zeros.  Keys whose scores are all -inf: 0 / 0, as the formula has it.)
+            const float f = p.n > p.lo ? 1.f / l : 0.f;
+            T* y = static_cast<T*>(a.out) + p.b * a.osb + (p.h0 + h) * a.osh + d;
+            const float v[4] = {o.x * f, o.y * f, o.z * f, o.w * f};
+            if (vec && d + 4 <= a.D) {
+                T t[4];
+                for (int j = 0; j < 4; ++j) t[j] = from_f32<T>(v[j]);
+                if (sizeof(T) == 2) *reinterpret_cast<uint2*>(y) = *reinterpret_cast<uint2*>(t);
+                else *reinterpret_cast<uint4*>(y) = *reinterpret_cast<uint4*>(t);
+            } else {
+                for (int j = 0; j < 4; ++j) if (d + j < a.D) y[j] = from_f32<T>(v[j]);
+            }
+            if (d == 0 && a.lse) a.lse[(int64_t)p.b * a.Hq + p.h0 + h] = (m + log2f(l)) * 0.69314718055994531f;
+        } else {
+            *reinterpret_cast<float4*>(a.part + (slot * HP + h) * DP + d) = o;
+            if (d == 0) a.part_ml[slot * HP + h] = make_float2(m, l);
+        }
+    }
+    if (threadIdx.x == 0 && p.c0 == 0 && !whole) {
+        const int64_t last_unit = r.at - p.c1 + p.units - 1;        // (r.at is behind this piece)
+        int w = (int)(last_unit * gridDim.x / r.units);
+        while (w + 1 < (int)gridDim.x && run_start(r.units, w + 1, gridDim.x) <= last_unit) ++w;
+        while (run_start(r.units, w, gridDim.x) > last_unit) --w;
+        a.open[blockIdx.x] = Open{r.units, p.b, p.hg, w, 0};
+    }
+}
+
+// ---- tensor cores: 16-bit caches on 16-byte boundaries, heads of up to 256 values in eights --------------------------------
+template <typename T> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 ld16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    T t[2] = {from_f32<T>(lo), from_f32<T>(hi)};
+    return *reinterpret_cast<uint32_t*>(t);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x) {
+    const T* t = reinterpret_cast<const T*>(&x);
+    return make_float2(to_f32<T>(t[0]), to_f32<T>(t[1]));
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// Where the 16 rows of a tile lie.  IN_PAGE (page size a multiple of 16, or no table): one page and slot.  Else: lane r holds
+// those of row r.  Looked up a batch of tiles at a time, and the batch after it already, so that no tile waits for the table.
+template <bool IN_PAGE> struct Pages {
+    static constexpr int kBatch = IN_PAGE ? 32 : 2;      // units per batch
+    int id, slot, next_id, next_slot;                    // of this lane's tile or row
+    __device__ void fetch(const AttnArgs& a, const Piece& p, int c, int warp, int& page, int& at) const {
+        const int lane = threadIdx.x & 31;
+        const int unit = c + (IN_PAGE ? lane : lane >> 4);
+        const int64_t pos = (int64_t)p.base + ((int64_t)unit * kWarps + warp) * kTile + (IN_PAGE ? 0 : lane & 15);
+        page = -1;
+        at = 0;
+        if (unit < p.c1 && pos < p.n && (IN_PAGE || pos >= p.lo)) {
+            if (!a.table) {
+                page = p.b; at = (int)pos;
+                return;
+            }
+            const int i = (int)((uint32_t)pos / (uint32_t)a.page_size);
+            at = (int)pos - i * a.page_size;
+            page = a.table[p.b * a.ts + i];
+            if (page < 0 || page >= a.num_pages) {
+                atomicCAS(&g_device_status, 0, kStatusBadPage);
+                page = -1;
+            }
+        }
+    }
+};
+
+template <typename T, int DP, int NT, bool IN_PAGE> struct Tile {
+    // rows: keys 0..15 of the tile; mask: which of them count
+    uint32_t mask;
+    int64_t ko, vo;                       // IN_PAGE: offset of row 0
+    int64_t krow[2], vrow[4];             // else: offsets of the lane's rows
+};
+
+constexpr int decode_blocks_per_sm(int DP, int NT) { return DP == 64 ? (NT == 1 ? 5 : 4) : DP == 128 ? (NT == 1 ? 3 : 2) : 2; }
+
+template <typename T, int DP, int NT, bool IN_PAGE>
+__global__ void __launch_bounds__(kThreads, decode_blocks_per_sm(DP, NT)) decode_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int HP = 8 * NT, KC = DP / 32, VC = DP / 64, MT = DP / 16, PITCH = DP + 4;
+    __shared__ __align__(16) float s_o[kWarps * HP * PITCH];
+    __shared__ float s_m[kWarps][HP], s_l[kWarps][HP];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    if (threadIdx.x == 0) a.open[blockIdx.x].b = -1;
+    Run run(a);
+    const T* kp = static_cast<const T*>(a.k);
+    const T* vp = static_cast<const T*>(a.v);
+    const bool full_d = a.D == DP;
+    while (run.at < run.end) {
+        const Piece p = next_piece<HP>(a, run);
+        uint4 qf[KC][NT];
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int h = nt * 8 + g, d = i * 32 + t * 8;
+                qf[i][nt] = make_uint4(0, 0, 0, 0);
+                if (h < p.heads && d < a.D)
+                    qf[i][nt] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + p.b * a.qsb + (p.h0 + h) * a.qsh + d);
+            }
+        float m[NT][2], l[NT][2], o[MT][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -FLT_MAX;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+        }
+        const T* kh = kp + p.kvh * a.ksh + t * 8;
+        const T* vh = vp + p.kvh * a.vsh + g * 8;
+        uint4 kr[KC][2], vr[VC][4];
+        Pages<IN_PAGE> pages;
+        pages.fetch(a, p, p.c0, warp, pages.id, pages.slot);
+        pages.fetch(a, p, p.c0 + pages.kBatch, warp, pages.next_id, pages.next_slot);
+        int left = pages.kBatch;
+
+        // rows of unit c's tile; moves the lookups on
+        auto locate = [&](int c) {
+            Tile<T, DP, NT, IN_PAGE> tl;
+            if (left == 0) {
+                pages.id = pages.next_id; pages.slot = pages.next_slot;
+                pages.fetch(a, p, c + pages.kBatch, warp, pages.next_id, pages.next_slot);
+                left = pages.kBatch;
+            }
+            const int j = pages.kBatch - left--;
+            const int64_t pos = (int64_t)p.base + ((int64_t)c * kWarps + warp) * kTile;
+            if (IN_PAGE) {
+                const int id = __shfl_sync(0xffffffffu, pages.id, j), slot = __shfl_sync(0xffffffffu, pages.slot, j);
+                tl.mask = 0;
+                if (id >= 0) {
+                    const int64_t from = p.lo - pos, to = p.n - pos;          // rows from .. to - 1
+                    tl.mask = to >= 16 ? 0xffffu : (1u << to) - 1u;            // (to > 0 where there is a page)
+                    if (from > 0) tl.mask &= from >= 16 ? 0u : 0xffffu << from;
+                }
+                tl.ko = (int64_t)id * a.ksp + (int64_t)slot * a.kss;
+                tl.vo = (int64_t)id * a.vsp + (int64_t)slot * a.vss;
+            } else {
+                const int at = j * 16;
+                tl.mask = (__ballot_sync(0xffffffffu, pages.id >= 0) >> at) & 0xffffu;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = at + g + 8 * i;
+                    tl.krow[i] = (int64_t)__shfl_sync(0xffffffffu, pages.id, r) * a.ksp + (int64_t)__shfl_sync(0xffffffffu, pages.slot, r) * a.kss;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = at + 2 * t + (i & 1) + 8 * (i >> 1);
+                    tl.vrow[i] = (int64_t)__shfl_sync(0xffffffffu, pages.id, r) * a.vsp + (int64_t)__shfl_sync(0xffffffffu, pages.slot, r) * a.vss;
+                }
+            }
+            return tl;
+        };
+        // Rows that do not count are not read, and enter as zeros: whatever lies there stays out.
+        auto load_k = [&](const Tile<T, DP, NT, IN_PAGE>& tl) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const T* row = kh + (IN_PAGE ? tl.ko + (g + 8 * r) * a.kss : tl.krow[r]);
+                if (tl.mask == 0xffffu && full_d) {
+#pragma unroll
+                    for (int i = 0; i < KC; ++i) kr[i][r] = ld16(row + i * 32);
+                } else {
+                    const bool ok = (tl.mask >> (g + 8 * r)) & 1;
+#pragma unroll
+                    for (int i = 0; i < KC; ++i) {
+                        kr[i][r] = make_uint4(0, 0, 0, 0);
+                        if (ok && i * 32 + t * 8 < a.D) kr[i][r] = ld16(row + i * 32);
+                    }
+                }
+            }
+        };
+        auto load_v = [&](const Tile<T, DP, NT, IN_PAGE>& tl) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = 2 * t + (r & 1) + 8 * (r >> 1);
+                const T* row = vh + (IN_PAGE ? tl.vo + key * a.vss : tl.vrow[r]);
+                if (tl.mask == 0xffffu && full_d) {
+#pragma unroll
+                    for (int i = 0; i < VC; ++i) vr[i][r] = ld16(row + i * 64);
+                } else {
+                    const bool ok = (tl.mask >> key) & 1;
+#pragma unroll
+                    for (int i = 0; i < VC; ++i) {
+                        vr[i][r] = make_uint4(0, 0, 0, 0);
+                        if (ok && i * 64 + g * 8 < a.D) vr[i][r] = ld16(row + i * 64);
+                    }
+                }
+            }
+        };
+
+        Tile<T, DP, NT, IN_PAGE> cur = locate(p.c0);
+        load_k(cur);
+        load_v(cur);
+        for (int c = p.c0; c < p.c1; ++c) {
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+                for (int i = 0; i < KC; ++i) {
+                    mma<T>(s[nt], kr[i][0].x, kr[i][1].x, kr[i][0].y, kr[i][1].y, qf[i][nt].x, qf[i][nt].y);
+                    mma<T>(s[nt], kr[i][0].z, kr[i][1].z, kr[i][0].w, kr[i][1].w, qf[i][nt].z, qf[i][nt].w);
+                }
+            }
+            Tile<T, DP, NT, IN_PAGE> nxt;
+            const bool more = c + 1 < p.c1;
+            if (more) {
+                nxt = locate(c + 1);
+                load_k(nxt);
+            }
+            bool up = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][i] *= a.scale;
+                if (cur.mask != 0xffffu) {
+                    if (!((cur.mask >> g) & 1)) s[nt][0] = s[nt][1] = -INFINITY;
+                    if (!((cur.mask >> (g + 8)) & 1)) s[nt][2] = s[nt][3] = -INFINITY;
+                }
+                constexpr float over = Ref<T>::shift + Ref<T>::slack;
+                up |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + over || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + over;
+            }
+            if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float x = fmaxf(s[nt][i], s[nt][i + 2]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        x = fmaxf(x - Ref<T>::shift, m[nt][i]);
+                        const float f = exp2f(m[nt][i] - x);
+                        m[nt][i] = x;
+                        l[nt][i] *= f;
+#pragma unroll
+                        for (int j = 0; j < MT; ++j) { o[j][nt][i] *= f; o[j][nt][i + 2] *= f; }
+                    }
+            }
+            uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float p0 = exp2f(s[nt][2 * i] - m[nt][0]), p1 = exp2f(s[nt][2 * i + 1] - m[nt][1]);
+                    l[nt][0] += p0;
+                    l[nt][1] += p1;
+                    const uint32_t hi = pack2<T>(p0, p1);
+                    const float2 back = unpack2<T>(hi);
+                    ph[nt][i] = transpose8(hi);
+                    pl[nt][i] = transpose8(pack2<T>(p0 - back.x, p1 - back.y));
+                }
+#pragma unroll
+            for (int i = 0; i < VC; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t r0 = word(vr[i][0], j), r1 = word(vr[i][1], j), r2 = word(vr[i][2], j), r3 = word(vr[i][3], j);
+                    const uint32_t a0 = __byte_perm(r0, r1, 0x5410), a1 = __byte_perm(r0, r1, 0x7632);
+                    const uint32_t a2 = __byte_perm(r2, r3, 0x5410), a3 = __byte_perm(r2, r3, 0x7632);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma<T>(o[i * 4 + j][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                        mma<T>(o[i * 4 + j][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                    }
+                }
+            if (more) {
+                load_v(nxt);
+                cur = nxt;
+            }
+        }
+
+        __syncthreads();                                            // (the previous piece's sums have been read)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x = l[nt][i];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const int h = nt * 8 + 2 * t + i;
+                if (g == 0) { s_m[warp][h] = m[nt][i]; s_l[warp][h] = x; }
+                float* row = s_o + (warp * HP + h) * PITCH + g * 8;
+#pragma unroll
+                for (int v = 0; v < VC; ++v) {
+                    *reinterpret_cast<float4*>(row + v * 64) = make_float4(o[v * 4][nt][i], o[v * 4][nt][i + 2], o[v * 4 + 1][nt][i], o[v * 4 + 1][nt][i + 2]);
+                    *reinterpret_cast<float4*>(row + v * 64 + 4) = make_float4(o[v * 4 + 2][nt][i], o[v * 4 + 2][nt][i + 2], o[v * 4 + 3][nt][i], o[v * 4 + 3][nt][i + 2]);
+                }
+            }
+        __syncthreads();
+        join_warps<T, DP, HP, PITCH>(a, p, run, s_o, s_m, s_l, true);
+    }
+}
+
+// ---- any type, head size and alignment: fp32 products on the CUDA cores ----------------------------------------------------
+// Eight lanes hold a key, a lane the values 32 i + 4 (lane % 8) .. + 3 of it; a warp works on four keys at a time, each group
+// of eight lanes with a maximum and sums of its own.  Up to four query heads at a time.
+template <typename T, bool VEC> __device__ __forceinline__ float4 load4(const T* p, int d, int D) {
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (VEC) {
+        if (d < D) {
+            if (sizeof(T) == 4) return *reinterpret_cast<const float4*>(p + d);
+            const uint2 u = *reinterpret_cast<const uint2*>(p + d);
+            const T* t = reinterpret_cast<const T*>(&u);
+            r = make_float4(to_f32<T>(t[0]), to_f32<T>(t[1]), to_f32<T>(t[2]), to_f32<T>(t[3]));
+        }
+    } else {
+        if (d < D) r.x = to_f32<T>(p[d]);
+        if (d + 1 < D) r.y = to_f32<T>(p[d + 1]);
+        if (d + 2 < D) r.z = to_f32<T>(p[d + 2]);
+        if (d + 3 < D) r.w = to_f32<T>(p[d + 3]);
+    }
+    return r;
+}
+
+template <typename T, int DP, int HP, bool VEC>
+__global__ void __launch_bounds__(kThreads) decode_any_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int C = DP / 32, PITCH = DP + 4, STEPS = DP <= 128 ? 2 : 1;
+    __shared__ __align__(16) float s_o[kWarps * HP * PITCH], s_q[HP * DP];
+    __shared__ float s_m[kWarps][HP], s_l[kWarps][HP];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & 7, kq = lane >> 3;
+    if (threadIdx.x == 0) a.open[blockIdx.x].b = -1;
+    Run run(a);
+    while (run.at < run.end) {
+        const Piece p = next_piece<HP>(a, run);
+        __syncthreads();
+        for (int i = threadIdx.x; i < HP * DP; i += kThreads) {
+            const int h = i / DP, d = i - h * DP;
+            s_q[i] = h < p.heads && d < a.D ? to_f32<T>(static_cast<const T*>(a.q)[p.b * a.qsb + (p.h0 + h) * a.qsh + d]) : 0.f;
+        }
+        __syncthreads();
+        float m[HP], l[HP];
+        float4 o[HP][C];
+#pragma unroll
+        for (int h = 0; h < HP; ++h) {
+            m[h] = -FLT_MAX;
+            l[h] = 0.f;
+#pragma unroll
+            for (int i = 0; i < C; ++i) o[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const T* kh = static_cast<const T*>(a.k) + p.kvh * a.ksh;
+        const T* vh = static_cast<const T*>(a.v) + p.kvh * a.vsh;
+        for (int c = p.c0; c < p.c1; ++c) {
+            for (int step = 0; step < kTile / 4; step += STEPS) {
+                float4 kv[STEPS][C], vv[STEPS][C];
+                bool ok[STEPS];
+#pragma unroll
+                for (int u = 0; u < STEPS; ++u) {
+                    const int64_t pos = (int64_t)p.base + ((int64_t)c * kWarps + warp) * kTile + (step + u) * 4 + kq;
+                    int page = p.b, at = (int)pos;
+                    ok[u] = pos >= p.lo && pos < p.n;
+                    if (ok[u] && a.table) {
+                        const int i = (int)((uint32_t)pos / (uint32_t)a.page_size);
+                        at = (int)pos - i * a.page_size;
+                        page = a.table[p.b * a.ts + i];
+                        if (page < 0 || page >= a.num_pages) {
+                            atomicCAS(&g_device_status, 0, kStatusBadPage);
+                            ok[u] = false;
+                        }
+                    }
+                    const T* kk = kh + page * a.ksp + at * a.kss;
+                    const T* vk = vh + page * a.vsp + at * a.vss;
+#pragma unroll
+                    for (int i = 0; i < C; ++i) {
+                        kv[u][i] = vv[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (ok[u]) {
+                            kv[u][i] = load4<T, VEC>(kk, i * 32 + sub * 4, a.D);
+                            vv[u][i] = load4<T, VEC>(vk, i * 32 + sub * 4, a.D);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+                    for (int h = 0; h < HP; ++h) {
+                        float s = 0.f;
+#pragma unroll
+                        for (int i = 0; i < C; ++i) {
+                            const float4 q = *reinterpret_cast<const float4*>(s_q + h * DP + i * 32 + sub * 4);
+                            s += q.x * kv[u][i].x + q.y * kv[u][i].y + q.z * kv[u][i].z + q.w * kv[u][i].w;
+                        }
+                        s += __shfl_xor_sync(0xffffffffu, s, 1);
+                        s += __shfl_xor_sync(0xffffffffu, s, 2);
+                        s += __shfl_xor_sync(0xffffffffu, s, 4);
+                        s = ok[u] ? s * a.scale : -INFINITY;
+                        if (s > m[h] + Ref<float>::slack) {
+                            const float f = exp2f(m[h] - s);
+                            m[h] = s;
+                            l[h] *= f;
+#pragma unroll
+                            for (int i = 0; i < C; ++i) { o[h][i].x *= f; o[h][i].y *= f; o[h][i].z *= f; o[h][i].w *= f; }
+                        }
+                        const float e = exp2f(s - m[h]);
+                        l[h] += e;
+#pragma unroll
+                        for (int i = 0; i < C; ++i) {
+                            o[h][i].x += e * vv[u][i].x; o[h][i].y += e * vv[u][i].y;
+                            o[h][i].z += e * vv[u][i].z; o[h][i].w += e * vv[u][i].w;
+                        }
+                    }
+            }
+        }
+        // the four groups of a warp, then the warps
+#pragma unroll
+        for (int h = 0; h < HP; ++h) {
+            float x = fmaxf(m[h], __shfl_xor_sync(0xffffffffu, m[h], 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float f = exp2f(m[h] - x);
+            auto sum = [&](float v) {
+                v *= f;
+                v += __shfl_xor_sync(0xffffffffu, v, 8);
+                return v + __shfl_xor_sync(0xffffffffu, v, 16);
+            };
+            const float lt = sum(l[h]);
+            if (lane == 0) { s_m[warp][h] = x; s_l[warp][h] = lt; }
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const float4 r = make_float4(sum(o[h][i].x), sum(o[h][i].y), sum(o[h][i].z), sum(o[h][i].w));
+                if (kq == 0) *reinterpret_cast<float4*>(s_o + (warp * HP + h) * PITCH + i * 32 + sub * 4) = r;
+            }
+        }
+        __syncthreads();
+        join_warps<T, DP, HP, PITCH>(a, p, run, s_o, s_m, s_l, false);
+    }
+}
+
+// ---- the open (sequence, head group)s: block (w, h) joins head h of the one that begins in run w ----------------------------
+template <typename T, int DP, int HP> __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ AttnArgs a, int W) {
+    constexpr int Q = DP / 4, R = kThreads / Q;                      // threads to a row of sums; rows at a time
+    extern __shared__ float s_f[];                                   // [W] factors
+    __shared__ float s_red[2][kWarps];
+    __shared__ __align__(16) float s_o[R][DP];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int w0 = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Open op = a.open[w0];
+    if (op.b < 0) return;
+    const int kvh = op.hg / a.passes, first = (op.hg - kvh * a.passes) * HP;
+    if (first + h >= a.G) return;
+    const int n = op.last - w0 + 1;
+    // the run it begins in keeps it in slot 1, the others in slot 0; a run may be empty
+    auto row = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i == 0)) * HP + h; };
+    auto empty = [&](int i) { return run_start(op.units, w0 + i, W) == run_start(op.units, w0 + i + 1, W); };
+    float m = -FLT_MAX;
+    for (int i = tid; i < n; i += kThreads)
+        if (!empty(i)) m = fmaxf(m, a.part_ml[row(i)].x);
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s_red[0][warp] = m;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_red[0][w]);
+    float l = 0.f;
+    for (int i = tid; i < n; i += kThreads) {
+        float f = 0.f;
+        if (!empty(i)) {
+            const float2 ml = a.part_ml[row(i)];
+            f = exp2f(ml.x - m);
+            l += f * ml.y;
+        }
+        s_f[i] = f;
+    }
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) s_red[1][warp] = l;
+    __syncthreads();
+    l = 0.f;
+    for (int w = 0; w < kWarps; ++w) l += s_red[1][w];
+    const int q = tid % Q, r0 = tid / Q;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = r0; i < n; i += R) {
+        if (empty(i)) continue;
+        const float f = s_f[i];
+        const float4 x = *reinterpret_cast<const float4*>(a.part + row(i) * DP + q * 4);
+        o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+    }
+    *reinterpret_cast<float4*>(&s_o[r0][q * 4]) = o;
+    __syncthreads();
+    const int head = kvh * a.G + first + h;
+    T* y = static_cast<T*>(a.out) + op.b * a.osb + head * a.osh;
+    for (int d = tid; d < a.D; d += kThreads) {
+        float x = 0.f;
+        for (int i = 0; i < R; ++i) x += s_o[i][d];
+        y[d] = from_f32<T>(x / l);
+    }
+    if (tid == 0 && a.lse) a.lse[(int64_t)op.b * a.Hq + head] = (m + log2f(l)) * 0.69314718055994531f;
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+struct Plan {
+    int DP, HP, blocks;
+    bool tensor, in_page, vec;
+    int64_t slots, bytes;
+};
+
+bool aligned(const void* p, int64_t a, int64_t b, int64_t c, int64_t es, int64_t n) {
+    return reinterpret_cast<uintptr_t>(p) % n == 0 && (a * es) % n == 0 && (b * es) % n == 0 && (c * es) % n == 0;
+}
+
+Plan make_plan(const vtx_paged_decode_params& p) {
+    Plan pl{};
+    const int64_t es = dtype_size(p.io_dtype), G = p.Hq / p.Hk;
+    pl.DP = p.D <= 64 ? 64 : p.D <= 128 ? 128 : 256;
+    pl.tensor = es == 2 && p.D % 8 == 0 && aligned(p.q, p.q_stride_b, p.q_stride_h, 0, es, 16) &&
+                aligned(p.k_pages, p.k_stride_page, p.k_stride_slot, p.k_stride_head, es, 16) &&
+                aligned(p.v_pages, p.v_stride_page, p.v_stride_slot, p.v_stride_head, es, 16) &&
+                aligned(p.out, p.out_stride_b, p.out_stride_h, 0, es, 8);
+    pl.in_page = !p.block_table || p.page_size % kTile == 0;
+    pl.vec = p.D % 4 == 0 && aligned(p.k_pages, p.k_stride_page, p.k_stride_slot, p.k_stride_head, es, 4 * es) &&
+             aligned(p.v_pages, p.v_stride_page, p.v_stride_slot, p.v_stride_head, es, 4 * es);
+    int per_sm;
+    if (pl.tensor) {
+        // 9 to 16 query heads of a key head share a pass (but for heads of 256 values, whose sums fill the registers)
+        const int NT = G > 8 && pl.DP < 256 ? 2 : 1;
+        pl.HP = 8 * NT;
+        per_sm = decode_blocks_per_sm(pl.DP, NT);
+    } else {
+        pl.HP = G > 1 ? 4 : 1;
+        per_sm = 3;
+    }
+    // no more blocks than units
+    const int64_t keys = p.block_table ? p.table_width * p.page_size : p.page_size;
+    const int64_t per_seq = ceil_div<int64_t>(keys < INT32_MAX ? keys : INT32_MAX, kUnit) + 1;
+    const int64_t pairs = p.B * p.Hk * ceil_div<int64_t>(G, pl.HP);
+    int64_t most = pairs > (1 << 20) ? pairs : pairs * (per_seq > 0 ? per_seq : 1);
+    pl.blocks = (int)(most < (int64_t)kNumSMs * per_sm ? most : (int64_t)kNumSMs * per_sm);
+    pl.slots = (int64_t)pl.blocks * 2 * pl.HP;
+    pl.bytes = pl.slots * (pl.DP * 4 + 8) + (int64_t)pl.blocks * sizeof(Open);
+    return pl;
+}
+
+template <typename T, int DP, int HP> int launch_join(const AttnArgs& a, int W, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)W, (unsigned)(a.G < HP ? a.G : HP));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)W * sizeof(float);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, join_kernel<T, DP, HP>, a, W);
+    return check_launch("paged_decode_attention", 2);
+}
+
+template <typename T, int DP> int launch_tensor(const AttnArgs& a, const Plan& pl, cudaStream_t s) {
+    const unsigned W = (unsigned)pl.blocks;
+    if (pl.HP == 8) {
+        if (pl.in_page) decode_kernel<T, DP, 1, true><<<W, kThreads, 0, s>>>(a);
+        else decode_kernel<T, DP, 1, false><<<W, kThreads, 0, s>>>(a);
+        return launch_join<T, DP, 8>(a, (int)W, s);
+    }
+    if constexpr (DP < 256) {
+        if (pl.in_page) decode_kernel<T, DP, 2, true><<<W, kThreads, 0, s>>>(a);
+        else decode_kernel<T, DP, 2, false><<<W, kThreads, 0, s>>>(a);
+        return launch_join<T, DP, 16>(a, (int)W, s);
+    }
+    return fail(VTX_ERR_UNSUPPORTED, "paged_decode_attention: no kernel");
+}
+
+template <typename T, int DP> int launch_any(const AttnArgs& a, const Plan& pl, cudaStream_t s) {
+    const unsigned W = (unsigned)pl.blocks;
+    if (pl.HP == 1) {
+        if (pl.vec) decode_any_kernel<T, DP, 1, true><<<W, kThreads, 0, s>>>(a);
+        else decode_any_kernel<T, DP, 1, false><<<W, kThreads, 0, s>>>(a);
+        return launch_join<T, DP, 1>(a, (int)W, s);
+    }
+    if (pl.vec) decode_any_kernel<T, DP, 4, true><<<W, kThreads, 0, s>>>(a);
+    else decode_any_kernel<T, DP, 4, false><<<W, kThreads, 0, s>>>(a);
+    return launch_join<T, DP, 4>(a, (int)W, s);
+}
+
+int validate(const vtx_paged_decode_params* p) {
+    VTX_REQUIRE(p, VTX_ERR_BAD_ARG, "paged_decode_attention: null pointer");
+    VTX_REQUIRE(valid_dtype(p->io_dtype), VTX_ERR_BAD_ARG, "paged_decode_attention: unknown io dtype %lld", (long long)p->io_dtype);
+    VTX_REQUIRE(p->B >= 0 && p->Hk > 0 && p->Hq > 0 && p->D > 0 && p->page_size > 0 && p->num_pages >= 0 && p->table_width >= 0,
+                VTX_ERR_BAD_ARG, "paged_decode_attention: bad sizes");
+    VTX_REQUIRE(p->Hq % p->Hk == 0, VTX_ERR_BAD_ARG, "paged_decode_attention: %lld query heads for %lld key heads",
+                (long long)p->Hq, (long long)p->Hk);
+    VTX_REQUIRE(p->D <= 256, VTX_ERR_UNSUPPORTED, "paged_decode_attention: heads of %lld > 256 values", (long long)p->D);
+    VTX_REQUIRE(p->window >= 0, VTX_ERR_BAD_ARG, "paged_decode_attention: negative window");
+    VTX_REQUIRE(p->B < (1 << 24) && p->Hq < (1 << 16) && p->num_pages < INT32_MAX && p->page_size < INT32_MAX, VTX_ERR_UNSUPPORTED,
+                "paged_decode_attention: more than 2^24 sequences, 2^16 heads or 2^31 pages or slots");
+    VTX_REQUIRE(p->block_table || p->num_pages >= p->B, VTX_ERR_BAD_ARG, "paged_decode_attention: %lld sequences, %lld pages and no block table",
+                (long long)p->B, (long long)p->num_pages);
+    return VTX_OK;
+}
+
+}  // namespace
+}  // namespace vtx
+
+extern "C" int64_t vtx_paged_decode_scratch_bytes(const vtx_paged_decode_params* p) {
+    if (vtx::validate(p) != VTX_OK) return 0;
+    return p->B ? vtx::make_plan(*p).bytes : 0;
+}
+
+extern "C" int vtx_paged_decode_attention(const vtx_paged_decode_params* p, void* stream) {
+    using namespace vtx;
+    if (int rc = validate(p)) return rc;
+    if (p->B == 0) return VTX_OK;
+    VTX_REQUIRE(p->q && p->out && p->seqlens && (p->num_pages == 0 || (p->k_pages && p->v_pages)), VTX_ERR_BAD_ARG,
+                "paged_decode_attention: null pointer");
+    VTX_REQUIRE(p->scratch && reinterpret_cast<uintptr_t>(p->scratch) % 16 == 0, VTX_ERR_BAD_ARG,
+                "paged_decode_attention: scratch needed (vtx_paged_decode_scratch_bytes, 16-byte aligned)");
+    const Plan pl = make_plan(*p);
+    AttnArgs a{};
+    a.q = p->q; a.qsb = p->q_stride_b; a.qsh = p->q_stride_h;
+    a.k = p->k_pages; a.ksp = p->k_stride_page; a.kss = p->k_stride_slot; a.ksh = p->k_stride_head;
+    a.v = p->v_pages; a.vsp = p->v_stride_page; a.vss = p->v_stride_slot; a.vsh = p->v_stride_head;
+    a.table = p->block_table; a.ts = p->table_stride; a.lens = p->seqlens;
+    a.out = p->out; a.osb = p->out_stride_b; a.osh = p->out_stride_h; a.lse = p->lse;
+    char* w = static_cast<char*>(p->scratch);
+    a.part = reinterpret_cast<float*>(w);
+    a.part_ml = reinterpret_cast<float2*>(w + pl.slots * pl.DP * 4);
+    a.open = reinterpret_cast<Open*>(w + pl.slots * (pl.DP * 4 + 8));
+    a.scale = (float)(p->softmax_scale * 1.44269504088896340736);
+    a.window = p->window > 0 && p->window < INT32_MAX ? (int)p->window : INT32_MAX;
+    a.B = (int)p->B; a.Hq = (int)p->Hq; a.G = (int)(p->Hq / p->Hk); a.D = (int)p->D;
+    a.page_size = (int)p->page_size; a.num_pages = (int)p->num_pages;
+    a.passes = (a.G + pl.HP - 1) / pl.HP;
+    a.head_groups = (int)p->Hk * a.passes;
+    a.max_keys = p->block_table ? p->table_width * p->page_size : p->page_size;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (pl.tensor) {
+        if (p->io_dtype == VTX_BF16)
+            return pl.DP == 64 ? launch_tensor<__nv_bfloat16, 64>(a, pl, s) : pl.DP == 128 ? launch_tensor<__nv_bfloat16, 128>(a, pl, s)
+                                                                              : launch_tensor<__nv_bfloat16, 256>(a, pl, s);
+        return pl.DP == 64 ? launch_tensor<__half, 64>(a, pl, s) : pl.DP == 128 ? launch_tensor<__half, 128>(a, pl, s) : launch_tensor<__half, 256>(a, pl, s);
+    }
+    VTX_DISPATCH_IO(p->io_dtype, T, {
+        return pl.DP == 64 ? launch_any<T, 64>(a, pl, s) : pl.DP == 128 ? launch_any<T, 128>(a, pl, s) : launch_any<T, 256>(a, pl, s);
+    });
+    return VTX_OK;
+}

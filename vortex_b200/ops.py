@@ -598,3 +598,34 @@ def iir_fwd_noalloc(z_pre: torch.Tensor, log_poles, residues, bias, D: int, y: t
         B=B, L=L, D=D, round_kv=int(round_kv), io_dtype=_code(z_pre))
     with _on(z_pre):
         _lib.check(_lib.lib().vtx_iir_fwd_noalloc(C.byref(p), _stream(z_pre)))
+
+
+# ---------------------------------------------------------------------------------------------- attention layers
+def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, eps=1e-6, interleaved=False, scale=1.0):
+    """q [T, Hq, D] or [B, L, Hq, D], k alike (or None) -> both normed and turned; see ``attn_ops.qk_norm_rotary``."""
+    return _lib.host().qk_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, float(eps), bool(interleaved), float(scale))
+
+
+def qk_norm_rotary_bwd(dq, dk, q, k, positions, inv_freq, q_weight=None, k_weight=None, *, eps=1e-6, interleaved=False,
+                       scale=1.0):
+    """Gradients of the same call's outputs -> those of q, k and the weights (None where there is no such input)."""
+    return _lib.host().qk_norm_rotary_bwd(dq, dk, q, k, positions, inv_freq, q_weight, k_weight, float(eps), bool(interleaved),
+                                          float(scale))
+
+
+def rotary_append(q, k, v, positions, k_pages, v_pages, block_table, inv_freq=None, q_weight=None, k_weight=None, *,
+                  seq_ids=None, eps=1e-6, interleaved=False, scale=1.0):
+    """The same on the queries and keys of new tokens, keys and values stored in pages; see ``attn_ops.rotary_append``."""
+    return _lib.host().rotary_append(q, k, v, positions, k_pages, v_pages, block_table, inv_freq, q_weight, k_weight, seq_ids,
+                                     float(eps), bool(interleaved), float(scale))
+
+
+def paged_decode_attention(q, k_pages, v_pages, block_table, seqlens, *, softmax_scale=None, window=0, want_lse=False):
+    """q [B, Hq, D] against the pages of each sequence -> out [B, Hq, D] and lse fp32 [B, Hq] or None; see
+    ``attn_ops.paged_decode_attention``."""
+    return _lib.host().paged_decode_attention(q, k_pages, v_pages, block_table, seqlens, softmax_scale, int(window), bool(want_lse))
+
+
+def copy_pages(pools, src, dst) -> None:
+    """pool[dst[i]] = pool[src[i]] in every pool; see ``attn_ops.copy_pages``."""
+    _lib.host().copy_pages(pools, src, dst)
