@@ -12,6 +12,7 @@
 // position * inv_freq in 32 bits is off by 0.03 rad at position 2^20; what is left goes to sincospif.
 #include "attn.cuh"
 #include "tma.cuh"
+#include "umma.cuh"
 
 VTX_DEFINE_STATUS_READER()
 
@@ -47,11 +48,12 @@ struct RotArgs {
     // backward
     const void* dy[2];
     int64_t dyb[2], dyl[2], dyh[2];
-    float* dw_part;              // [blocks][2][D]
+    float* dw_part;              // rows of D: the queries' blocks, then the keys'
 };
 
 constexpr int kThreads = 256;
 constexpr int kMaxD = 512;
+constexpr int kFwdBlocks = 3, kFwdSteps = 2, kBwdPerSM = 2;
 constexpr int kBwdBlocks = kNumSMs * 4;
 
 __device__ __forceinline__ int64_t load_pos(const RotArgs& a, int64_t b, int64_t l) {
@@ -84,52 +86,43 @@ __device__ __forceinline__ int64_t slot_offset(const RotArgs& a, int64_t tok, in
     return page * a.r[which].db + (pos - at * a.page_size) * a.r[which].dl;
 }
 
-template <typename T> struct Vec {
-    static constexpr int N = 16 / sizeof(T);
-    __device__ static void unpack(const uint4& v, float* f) {
-        const T* p = reinterpret_cast<const T*>(&v);
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = to_f32<T>(p[i]);
-    }
-    __device__ static uint4 pack(const float* f) {
-        uint4 v;
-        T* p = reinterpret_cast<T*>(&v);
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = from_f32<T>(f[i]);
-        return v;
-    }
-};
+using umma::f32x2;
+using umma::add2;
+using umma::fma2;
+using umma::mul2;
+using umma::pk2;
+using umma::sub2;
+using umma::up2;
 
-// Two vectors of N values turned in place: pairs (xa[i], xb[i]) in the half layout, neighbours in the interleaved one.
-template <int N, bool INTER> __device__ __forceinline__ void rotate(float* xa, float* xb, const float2* cs) {
-    if (INTER) {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            const float a0 = xa[2 * i], a1 = xa[2 * i + 1], b0 = xb[2 * i], b1 = xb[2 * i + 1];
-            const float2 p = cs[i], q = cs[N / 2 + i];
-            xa[2 * i] = a0 * p.x - a1 * p.y; xa[2 * i + 1] = a0 * p.y + a1 * p.x;
-            xb[2 * i] = b0 * q.x - b1 * q.y; xb[2 * i + 1] = b0 * q.y + b1 * q.x;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float x = xa[i], y = xb[i];
-            xa[i] = x * cs[i].x - y * cs[i].y; xb[i] = x * cs[i].y + y * cs[i].x;
-        }
-    }
+template <typename T> __device__ __forceinline__ float low(uint32_t w);
+template <typename T> __device__ __forceinline__ float high(uint32_t w);
+template <> __device__ __forceinline__ float low<__nv_bfloat16>(uint32_t w) { return umma::bf_lo(w); }
+template <> __device__ __forceinline__ float high<__nv_bfloat16>(uint32_t w) { return umma::bf_hi(w); }
+template <> __device__ __forceinline__ float low<__half>(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))); }
+template <> __device__ __forceinline__ float high<__half>(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    T t[2] = {from_f32<T>(lo), from_f32<T>(hi)};
+    return *reinterpret_cast<uint32_t*>(t);
 }
-
 __device__ __forceinline__ float group_sum(float v, int lanes) {
     for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+__device__ __forceinline__ float sum2(f32x2 v) {
+    float a, b;
+    up2(v, a, b);
+    return a + b;
+}
 
-// What a thread of the vector kernels does in every row: two 16-byte vectors of a head, whose pairs are complete.
+// What a lane of the vector kernels holds of a head: N pairs (a[i], b[i]), two values to a 64-bit register and instruction
+// (the arithmetic, not the traffic, took the time before: 590 instructions a step of the backward pass).  They come from two
+// 16-byte vectors: a from the one and b from the other in the half layout, the even and the odd values of both in the
+// interleaved one, which makes all that follows the same for both.
 template <typename T, bool INTER> struct Lane {
-    static constexpr int N = Vec<T>::N;
+    static constexpr int N = 16 / sizeof(T), P = N / 2;
     int ea, eb;          // first elements of the two vectors
     bool on, turned;     // inside the head; inside its rotated part
-    float2 cs[N];
+    f32x2 c[P], s[P];
     __device__ Lane(const RotArgs& a, int sub) {
         on = sub * 2 * N < a.D;
         turned = sub * 2 * N < a.rot;
@@ -141,206 +134,336 @@ template <typename T, bool INTER> struct Lane {
             ea = a.rot + (sub * 2 * N - a.rot) / 2; eb = ea + (a.D - a.rot) / 2;
         }
     }
-    __device__ void load_turns(const float2* row, int sub) {
-        if (turned)
+    // element of the head that value i of the 2N holds (a first, then b)
+    __device__ int element(int i) const { return INTER ? ea + 2 * (i < N ? i : i - N) + (i >= N) : i < N ? ea + i : eb + i - N; }
+    // cosines of a token's pairs, then their sines
+    __device__ void load_turns(const float* turns, int half, int sub) {
+        if (!turned) return;
 #pragma unroll
-            for (int i = 0; i < N; ++i) cs[i] = row[sub * N + i];
+        for (int i = 0; i < P; ++i) {
+            c[i] = *reinterpret_cast<const f32x2*>(turns + sub * N + 2 * i);
+            s[i] = *reinterpret_cast<const f32x2*>(turns + half + sub * N + 2 * i);
+        }
+    }
+    __device__ static void unpack(const uint4& u, const uint4& v, f32x2* a, f32x2* b) {
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
+        if constexpr (sizeof(T) == 4) {
+            auto f = [](uint32_t w) { return __uint_as_float(w); };
+            if (INTER) {
+                a[0] = pk2(f(x[0]), f(x[2])); b[0] = pk2(f(x[1]), f(x[3]));
+                a[1] = pk2(f(y[0]), f(y[2])); b[1] = pk2(f(y[1]), f(y[3]));
+            } else {
+                a[0] = pk2(f(x[0]), f(x[1])); a[1] = pk2(f(x[2]), f(x[3]));
+                b[0] = pk2(f(y[0]), f(y[1])); b[1] = pk2(f(y[2]), f(y[3]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (INTER) {
+                    const uint32_t p = i < 2 ? x[2 * i] : y[2 * i - 4], q = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
+                    a[i] = pk2(low<T>(p), low<T>(q)); b[i] = pk2(high<T>(p), high<T>(q));
+                } else {
+                    a[i] = pk2(low<T>(x[i]), high<T>(x[i])); b[i] = pk2(low<T>(y[i]), high<T>(y[i]));
+                }
+            }
+        }
+    }
+    __device__ static void pack(const f32x2* a, const f32x2* b, uint4& u, uint4& v) {
+        uint32_t x[4], y[4];
+        float a0, a1, b0, b1;
+        if constexpr (sizeof(T) == 4) {
+            auto w = [](float f) { return __float_as_uint(f); };
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                up2(a[i], a0, a1);
+                up2(b[i], b0, b1);
+                uint32_t* z = i ? y : x;
+                if (INTER) { z[0] = w(a0); z[1] = w(b0); z[2] = w(a1); z[3] = w(b1); }
+                else { x[2 * i] = w(a0); x[2 * i + 1] = w(a1); y[2 * i] = w(b0); y[2 * i + 1] = w(b1); }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                up2(a[i], a0, a1);
+                up2(b[i], b0, b1);
+                if (INTER) {
+                    uint32_t* z = i < 2 ? x + 2 * i : y + 2 * i - 4;
+                    z[0] = pack2<T>(a0, b0); z[1] = pack2<T>(a1, b1);
+                } else {
+                    x[i] = pack2<T>(a0, a1); y[i] = pack2<T>(b0, b1);
+                }
+            }
+        }
+        u = make_uint4(x[0], x[1], x[2], x[3]);
+        v = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+    __device__ void rotate(f32x2* a, f32x2* b) const {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const f32x2 x = a[i], y = b[i];
+            a[i] = sub2(mul2(x, c[i]), mul2(y, s[i]));
+            b[i] = fma2(x, s[i], mul2(y, c[i]));
+        }
     }
 };
 
-// Block: `tb` tokens, 256 threads = rows of `lanes` threads (a power of two that covers a head); the rows of a token take its
-// heads in turn.  Four heads' loads are issued before the first is used.
-template <typename T, bool INTER>
-__global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const __grid_constant__ RotArgs a, int tb, int lane_shift) {
-    constexpr int N = Vec<T>::N, U = 4;
-    extern __shared__ float2 s_cs[];                               // [tb][rot / 2]
-    __shared__ float s_w[2][kMaxD];
-    __shared__ int64_t s_slot[8][2];
-    const int tid = threadIdx.x, lanes = 1 << lane_shift, sub = tid & (lanes - 1), row = tid >> lane_shift;
-    const int per_token = (kThreads >> lane_shift) / tb, ti = row / per_token, slot = row - ti * per_token;
-    const int64_t T0 = (int64_t)blockIdx.x * tb, tokens = a.B * a.L;
+// The weights as the lanes hold them, in shared memory: quad q of a lane's 2N values at [q][lane], so that the lanes of a head
+// read neighbouring 16 bytes.
+template <typename T, bool INTER> __device__ __forceinline__ void stage_weights(const RotArgs& a, const Rows& r, float* dst, int lanes) {
+    constexpr int N = Lane<T, INTER>::N;
+    for (int i = threadIdx.x; i < 2 * N * lanes; i += kThreads) {
+        const int q = i / (4 * lanes), sub = i / 4 - q * lanes;
+        const Lane<T, INTER> ln(a, sub);
+        dst[i] = ln.on && r.w ? ld_param(r.w, r.wd, ln.element(q * 4 + (i & 3))) : 1.f;
+    }
+}
+__device__ __forceinline__ void load_quad(const float* w, int q, int lanes, int sub, f32x2& w0, f32x2& w1) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(w + (q * lanes + sub) * 4);
+    w0 = v.x;
+    w1 = v.y;
+}
+
+// Cosines and sines of a token's pairs, in the warp's piece of shared memory.
+__device__ __forceinline__ void warp_turns(const RotArgs& a, float* mine, int64_t pos) {
     const int half = a.rot / 2;
-    for (int i = tid; i < tb * half; i += kThreads) {
-        const int t = i / half;
-        const int64_t tok = T0 + t;
-        if (tok < tokens) s_cs[i] = turn(a, load_pos(a, tok / a.L, tok % a.L), i - t * half);
+    __syncwarp();
+    for (int i = threadIdx.x & 31; i < half; i += 32) {
+        const float2 cs = turn(a, pos, i);
+        mine[i] = cs.x;
+        mine[half + i] = cs.y;
     }
-    for (int i = tid; i < 2 * a.D; i += kThreads) {
-        const int which = i >= a.D;
-        if (a.r[which].w) s_w[which][i - which * a.D] = ld_param(a.r[which].w, a.r[which].wd, i - which * a.D);
-    }
-    if (a.paged && tid < 2 * tb && T0 + tid / 2 < tokens)
-        s_slot[tid / 2][tid & 1] = slot_offset(a, T0 + tid / 2, load_pos(a, (T0 + tid / 2) / a.L, (T0 + tid / 2) % a.L), 1 + (tid & 1));
-    __syncthreads();
-    Lane<T, INTER> ln(a, sub);
-    const int64_t tok = T0 + ti;
-    const bool live = ln.on && tok < tokens;
-    if (live) ln.load_turns(s_cs + ti * half, sub);
-    const int64_t b = live ? tok / a.L : 0, l = live ? tok - b * a.L : 0;
-    const int heads = a.r[0].H + a.r[1].H + a.r[2].H;
-    for (int h0 = 0; h0 < heads; h0 += per_token * U) {
-        uint4 va[U], vb[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            int h = h0 + u * per_token + slot;
-            va[u] = vb[u] = make_uint4(0, 0, 0, 0);
-            if (live && h < heads) {
-                const int which = h < a.r[0].H ? 0 : h < a.r[0].H + a.r[1].H ? 1 : 2;
-                h -= which == 0 ? 0 : which == 1 ? a.r[0].H : a.r[0].H + a.r[1].H;
-                const Rows& r = a.r[which];
-                const T* p = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + h * r.sh;
-                va[u] = *reinterpret_cast<const uint4*>(p + ln.ea);
-                vb[u] = *reinterpret_cast<const uint4*>(p + ln.eb);
-            }
+    __syncwarp();
+}
+
+// A warp takes one token and `chunk` heads of its queries, keys or values, 32 >> lane_shift heads side by side
+// (1 << lane_shift lanes cover a head), U steps in flight: a step's registers are refilled as soon as its values have been
+// unpacked.  No warp waits for another (but for the weights, once): a token's chain position -> angles, page lookup -> store
+// hides behind the other warps' traffic.
+struct Chunks { int size, q, k, v; };      // heads in one; chunks of a token's queries, keys, values
+
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(kThreads, kFwdBlocks) rotary_fwd_kernel(const __grid_constant__ RotArgs a, Chunks ch, int lane_shift) {
+    using Ln = Lane<T, INTER>;
+    constexpr int N = Ln::N, P = Ln::P, U = kFwdSteps;
+    extern __shared__ __align__(16) float s_turn[];                // [warp][rot]
+    __shared__ __align__(16) float s_w[2][kMaxD];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lanes = 1 << lane_shift, sub = lane & (lanes - 1), slot = lane >> lane_shift;
+    const int step = 32 >> lane_shift;
+    const bool any_norm = a.r[0].w || a.r[1].w;
+    const uint32_t item = blockIdx.x * (kThreads / 32) + warp, per = ch.q + ch.k + ch.v, tok = item / per, L = (uint32_t)a.L;
+    const bool live = tok < (uint32_t)(a.B * a.L);
+    int c = (int)(item - tok * per);
+    const int which = c < ch.q ? 0 : c < ch.q + ch.k ? 1 : 2;
+    c -= which == 0 ? 0 : which == 1 ? ch.q : ch.q + ch.k;
+    const Rows& r = a.r[which];
+    const uint32_t b = live ? tok / L : 0, l = live ? tok - b * L : 0;
+    const int first = c * ch.size, count = live ? (ch.size < r.H - first ? ch.size : r.H - first) : 0;
+    Ln ln(a, sub);
+    const T* src = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + (first + slot) * r.sh;
+    const int64_t src_step = step * r.sh;
+    uint4 va[U], vb[U];
+    int fh = slot;                                                 // head of the next step to fetch
+    auto fetch = [&](int u) {
+        va[u] = vb[u] = make_uint4(0, 0, 0, 0);
+        if (ln.on && fh < count) {
+            va[u] = *reinterpret_cast<const uint4*>(src + ln.ea);
+            vb[u] = *reinterpret_cast<const uint4*>(src + ln.eb);
         }
+        src += src_step;
+        fh += step;
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch(u);
+    if (any_norm) {
+        stage_weights<T, INTER>(a, a.r[0], s_w[0], lanes);
+        stage_weights<T, INTER>(a, a.r[1], s_w[1], lanes);
+        __syncthreads();
+    }
+    if (!live) return;
+    const int64_t pos = load_pos(a, b, l);
+    int64_t at = b * r.db + l * r.dl;
+    if (a.paged && which) {
+        at = slot_offset(a, tok, pos, which);
+        if (at < 0) return;
+    }
+    T* dst = static_cast<T*>(r.dst) + at + (first + slot) * r.dh;
+    const int64_t dst_step = step * r.dh;
+    if (which < 2) {
+        warp_turns(a, s_turn + warp * a.rot, pos);
+        ln.load_turns(s_turn + warp * a.rot, a.rot / 2, sub);
+    }
+    const bool norm = which < 2 && r.w;
+    for (int h0 = 0; h0 < count;) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            int h = h0 + u * per_token + slot;
-            if (h0 + u * per_token >= heads) break;                // (the same for the whole block)
-            const bool mine = live && h < heads;
-            const int which = h < a.r[0].H ? 0 : h < a.r[0].H + a.r[1].H ? 1 : 2;
-            h -= which == 0 ? 0 : which == 1 ? a.r[0].H : a.r[0].H + a.r[1].H;
-            const Rows& r = a.r[which];
-            float xa[N], xb[N];
-            Vec<T>::unpack(va[u], xa);
-            Vec<T>::unpack(vb[u], xb);
-            if (a.r[0].w || a.r[1].w) {                            // (uniform: the lanes of a head meet)
-                float ss = 0.f;
+            if (h0 >= count) break;                                // (the same for the whole warp)
+            const bool mine = ln.on && h0 + slot < count;
+            uint4 ra = va[u], rb = vb[u];
+            fetch(u);
+            if (which < 2) {
+                f32x2 xa[P], xb[P];
+                Ln::unpack(ra, rb, xa, xb);
+                if (norm) {
+                    f32x2 ss2 = mul2(xa[0], xa[0]);
 #pragma unroll
-                for (int i = 0; i < N; ++i) ss += xa[i] * xa[i] + xb[i] * xb[i];
-                ss = group_sum(ss, lanes);
-                if (which < 2 && r.w && mine) {
+                    for (int i = 1; i < P; ++i) ss2 = fma2(xa[i], xa[i], ss2);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) ss2 = fma2(xb[i], xb[i], ss2);
+                    const float ss = group_sum(sum2(ss2), lanes);
                     const float inv = rsqrtf(ss / (float)a.D + a.eps);
+                    const f32x2 inv2 = pk2(inv, inv);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        xa[i] *= inv * s_w[which][ln.ea + i];
-                        xb[i] *= inv * s_w[which][ln.eb + i];
+                    for (int q = 0; q < N / 2; ++q) {
+                        f32x2 w0, w1;
+                        load_quad(s_w[which], q, lanes, sub, w0, w1);
+                        f32x2* x = q < N / 4 ? xa + 2 * q : xb + 2 * (q - N / 4);
+                        x[0] = mul2(mul2(x[0], inv2), w0);
+                        x[1] = mul2(mul2(x[1], inv2), w1);
                     }
                 }
+                if (ln.turned) ln.rotate(xa, xb);
+                Ln::pack(xa, xb, ra, rb);
             }
-            if (!mine) continue;
-            T* d = static_cast<T*>(r.dst) + h * r.dh;
-            if (a.paged && which) {
-                const int64_t at = s_slot[ti][which - 1];
-                if (at < 0) continue;
-                d += at;
-            } else {
-                d += b * r.db + l * r.dl;
+            if (mine) {
+                *reinterpret_cast<uint4*>(dst + ln.ea) = ra;
+                *reinterpret_cast<uint4*>(dst + ln.eb) = rb;
             }
-            if (which < 2) {
-                if (ln.turned) rotate<N, INTER>(xa, xb, ln.cs);
-                va[u] = Vec<T>::pack(xa);
-                vb[u] = Vec<T>::pack(xb);
-            }
-            *reinterpret_cast<uint4*>(d + ln.ea) = va[u];
-            *reinterpret_cast<uint4*>(d + ln.eb) = vb[u];
+            dst += dst_step;
+            h0 += step;
         }
     }
 }
 
-// Backward behind a norm.  The blocks walk the tokens; a thread keeps its dimensions through all rows, so the weights'
-// gradients gather in its registers, then across the block's rows, and leave as one row of partial sums per block: summed in
-// a fixed order, no atomics.
+// Backward behind a norm.  The first blocks take the queries, the rest the keys; a warp walks its tokens, all heads of one
+// before the next, U steps in flight across them.  A lane keeps its dimensions through all rows, so the weight's gradient
+// gathers in its registers, then across the block, and leaves as one row of partial sums per block: summed in a fixed order,
+// no atomics.
 template <typename T, bool INTER>
-__global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const __grid_constant__ RotArgs a, int tb, int lane_shift) {
-    constexpr int N = Vec<T>::N, U = 2;
-    extern __shared__ float2 s_cs[];                               // [tb][rot / 2], later the rows' sums [rows][D]
-    __shared__ float s_w[2][kMaxD];
-    const int tid = threadIdx.x, lanes = 1 << lane_shift, sub = tid & (lanes - 1), row = tid >> lane_shift;
-    const int rows = kThreads >> lane_shift, per_token = rows / tb, ti = row / per_token, slot = row - ti * per_token;
-    const int64_t tokens = a.B * a.L;
-    const int half = a.rot / 2;
-    for (int i = tid; i < 2 * a.D; i += kThreads) {
-        const int which = i >= a.D;
-        s_w[which][i - which * a.D] = a.r[which].w ? ld_param(a.r[which].w, a.r[which].wd, i - which * a.D) : 1.f;
-    }
-    Lane<T, INTER> ln(a, sub);
-    float dw[2][2 * N] = {};
-    for (int64_t T0 = (int64_t)blockIdx.x * tb; T0 < tokens; T0 += (int64_t)gridDim.x * tb) {
-        __syncthreads();
-        for (int i = tid; i < tb * half; i += kThreads) {
-            const int t = i / half;
-            const int64_t tok = T0 + t;
-            if (tok < tokens) s_cs[i] = turn(a, load_pos(a, tok / a.L, tok % a.L), i - t * half);
+__global__ void __launch_bounds__(kThreads, kBwdPerSM) rotary_bwd_kernel(const __grid_constant__ RotArgs a, int q_blocks, int lane_shift) {
+    using Ln = Lane<T, INTER>;
+    constexpr int N = Ln::N, P = Ln::P, U = 2;
+    extern __shared__ __align__(16) float s_turn[];                // [warp][rot], later the rows' sums [rows][D]
+    __shared__ __align__(16) float s_w[kMaxD];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lanes = 1 << lane_shift, sub = lane & (lanes - 1), slot = lane >> lane_shift;
+    const int step = 32 >> lane_shift, rows = kThreads >> lane_shift;
+    const int which = (int)blockIdx.x >= q_blocks;
+    const Rows& r = a.r[which];
+    const uint32_t tokens = (uint32_t)(a.B * a.L), L = (uint32_t)a.L;
+    const uint32_t w0 = (blockIdx.x - (which ? q_blocks : 0)) * (kThreads / 32) + warp;
+    const uint32_t warps = (which ? gridDim.x - q_blocks : q_blocks) * (kThreads / 32);
+    const bool norm = r.w;
+    Ln ln(a, sub);
+    f32x2 dwa[P], dwb[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) dwa[i] = dwb[i] = pk2(0.f, 0.f);
+    uint4 va[U], vb[U], ga[U], gb[U];
+    uint32_t ft = w0;                                              // token and first head of the next step to fetch
+    int fh = 0;
+    const T *xp = nullptr, *gp = nullptr;
+    const int64_t xstep = step * r.sh, gstep = step * a.dyh[which];
+    auto fetch = [&](int u) {
+        va[u] = vb[u] = ga[u] = gb[u] = make_uint4(0, 0, 0, 0);
+        if (fh == 0) {
+            const uint32_t b = ft / L, l = ft - b * L;
+            xp = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + slot * r.sh;
+            gp = static_cast<const T*>(a.dy[which]) + b * a.dyb[which] + l * a.dyl[which] + slot * a.dyh[which];
         }
-        __syncthreads();
-        const int64_t tok = T0 + ti;
-        const bool live = ln.on && tok < tokens;
-        if (live) ln.load_turns(s_cs + ti * half, sub);
-        const int64_t b = live ? tok / a.L : 0, l = live ? tok - b * a.L : 0;
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const Rows& r = a.r[which];
-            for (int h0 = 0; h0 < r.H; h0 += per_token * U) {
-                uint4 va[U], vb[U], ga[U], gb[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int h = h0 + u * per_token + slot;
-                    va[u] = vb[u] = ga[u] = gb[u] = make_uint4(0, 0, 0, 0);
-                    if (live && h < r.H) {
-                        const T* p = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + h * r.sh;
-                        const T* g = static_cast<const T*>(a.dy[which]) + b * a.dyb[which] + l * a.dyl[which] + h * a.dyh[which];
-                        va[u] = *reinterpret_cast<const uint4*>(p + ln.ea);
-                        vb[u] = *reinterpret_cast<const uint4*>(p + ln.eb);
-                        ga[u] = *reinterpret_cast<const uint4*>(g + ln.ea);
-                        gb[u] = *reinterpret_cast<const uint4*>(g + ln.eb);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int h = h0 + u * per_token + slot;
-                    float xa[N], xb[N], da[N], db[N];
-                    Vec<T>::unpack(va[u], xa);
-                    Vec<T>::unpack(vb[u], xb);
-                    Vec<T>::unpack(ga[u], da);
-                    Vec<T>::unpack(gb[u], db);
-                    if (ln.turned) rotate<N, INTER>(da, db, ln.cs);
-                    if (r.w) {
-                        float ss = 0.f, dot = 0.f;
-#pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            ss += xa[i] * xa[i] + xb[i] * xb[i];
-                            dot += s_w[which][ln.on ? ln.ea + i : 0] * da[i] * xa[i] + s_w[which][ln.on ? ln.eb + i : 0] * db[i] * xb[i];
-                        }
-                        ss = group_sum(ss, lanes);
-                        dot = group_sum(dot, lanes);
-                        const float inv = rsqrtf(ss / (float)a.D + a.eps);
-                        const float back = dot * inv * inv / (float)a.D;    // mean(w g xh) / r, to multiply x
-                        if (live && h < r.H) {
-#pragma unroll
-                            for (int i = 0; i < N; ++i) {
-                                dw[which][i] += da[i] * xa[i] * inv;
-                                dw[which][N + i] += db[i] * xb[i] * inv;
-                                da[i] = inv * (s_w[which][ln.ea + i] * da[i] - back * xa[i]);
-                                db[i] = inv * (s_w[which][ln.eb + i] * db[i] - back * xb[i]);
-                            }
-                        }
-                    }
-                    if (live && h < r.H) {
-                        T* d = static_cast<T*>(r.dst) + b * r.db + l * r.dl + h * r.dh;
-                        *reinterpret_cast<uint4*>(d + ln.ea) = Vec<T>::pack(da);
-                        *reinterpret_cast<uint4*>(d + ln.eb) = Vec<T>::pack(db);
-                    }
-                }
+        if (ln.on && ft < tokens && fh + slot < r.H) {
+            ga[u] = *reinterpret_cast<const uint4*>(gp + ln.ea);
+            gb[u] = *reinterpret_cast<const uint4*>(gp + ln.eb);
+            if (norm) {
+                va[u] = *reinterpret_cast<const uint4*>(xp + ln.ea);
+                vb[u] = *reinterpret_cast<const uint4*>(xp + ln.eb);
             }
         }
-    }
-    float* s_sum = reinterpret_cast<float*>(s_cs);
+        xp += xstep;
+        gp += gstep;
+        fh += step;
+        if (fh >= r.H) { fh = 0; ft = ft + warps < ft ? tokens : ft + warps; }
+    };
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        __syncthreads();
-        if (ln.on)
+    for (int u = 0; u < U; ++u) fetch(u);
+    stage_weights<T, INTER>(a, r, s_w, lanes);
+    __syncthreads();
+    uint32_t t = w0;
+    int h0 = 0;
+    T* dst = nullptr;
+    const int64_t dstep = step * r.dh;
+    while (t < tokens) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                s_sum[row * a.D + ln.ea + i] = dw[which][i];
-                s_sum[row * a.D + ln.eb + i] = dw[which][N + i];
+        for (int u = 0; u < U; ++u) {
+            if (t >= tokens) break;
+            if (h0 == 0) {
+                const uint32_t b = t / L, l = t - b * L;
+                warp_turns(a, s_turn + warp * a.rot, load_pos(a, b, l));
+                ln.load_turns(s_turn + warp * a.rot, a.rot / 2, sub);
+                dst = static_cast<T*>(r.dst) + b * r.db + l * r.dl + slot * r.dh;
             }
-        __syncthreads();
-        for (int d = tid; d < a.D; d += kThreads) {
-            float s = 0.f;
-            for (int i = 0; i < rows; ++i) s += s_sum[i * a.D + d];
-            a.dw_part[((int64_t)blockIdx.x * 2 + which) * a.D + d] = s;
+            f32x2 xa[P], xb[P], da[P], db[P];
+            Ln::unpack(va[u], vb[u], xa, xb);
+            Ln::unpack(ga[u], gb[u], da, db);
+            fetch(u);
+            if (ln.turned) ln.rotate(da, db);
+            if (norm) {
+                f32x2 ss2 = mul2(xa[0], xa[0]), dot2 = pk2(0.f, 0.f);
+#pragma unroll
+                for (int i = 1; i < P; ++i) ss2 = fma2(xa[i], xa[i], ss2);
+#pragma unroll
+                for (int i = 0; i < P; ++i) ss2 = fma2(xb[i], xb[i], ss2);
+                const float ss = group_sum(sum2(ss2), lanes);
+                const float inv = rsqrtf(ss / (float)a.D + a.eps);
+                const f32x2 inv2 = pk2(inv, inv);
+#pragma unroll
+                for (int q = 0; q < N / 2; ++q) {
+                    f32x2 wq[2];
+                    load_quad(s_w, q, lanes, sub, wq[0], wq[1]);
+                    const int at = q < N / 4 ? 2 * q : 2 * (q - N / 4);
+                    f32x2 *x = (q < N / 4 ? xa : xb) + at, *d = (q < N / 4 ? da : db) + at, *dw = (q < N / 4 ? dwa : dwb) + at;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        // (lanes outside the head and its rows hold zeros)
+                        x[j] = mul2(x[j], inv2);                            // xh
+                        dw[j] = fma2(d[j], x[j], dw[j]);
+                        d[j] = mul2(d[j], wq[j]);                           // w g
+                        dot2 = fma2(d[j], x[j], dot2);
+                    }
+                }
+                const float mean = group_sum(sum2(dot2), lanes) * (-1.f / (float)a.D);
+                const f32x2 mean2 = pk2(mean, mean);
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    da[i] = mul2(fma2(mean2, xa[i], da[i]), inv2);
+                    db[i] = mul2(fma2(mean2, xb[i], db[i]), inv2);
+                }
+            }
+            if (ln.on && h0 + slot < r.H) {
+                uint4 ra, rb;
+                Ln::pack(da, db, ra, rb);
+                *reinterpret_cast<uint4*>(dst + ln.ea) = ra;
+                *reinterpret_cast<uint4*>(dst + ln.eb) = rb;
+            }
+            dst += dstep;
+            h0 += step;
+            if (h0 >= r.H) { h0 = 0; t = t + warps < t ? tokens : t + warps; }
         }
+    }
+    float* s_sum = s_turn;
+    const int row = tid >> lane_shift;
+    __syncthreads();
+    if (ln.on)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float lo, hi;
+            up2(dwa[i / 2], lo, hi);
+            s_sum[row * a.D + ln.element(i)] = i & 1 ? hi : lo;
+            up2(dwb[i / 2], lo, hi);
+            s_sum[row * a.D + ln.element(N + i)] = i & 1 ? hi : lo;
+        }
+    __syncthreads();
+    for (int d = tid; d < a.D; d += kThreads) {
+        float sum = 0.f;
+        for (int i = 0; i < rows; ++i) sum += s_sum[i * a.D + d];
+        a.dw_part[(int64_t)blockIdx.x * a.D + d] = sum;
     }
 }
 
@@ -458,23 +581,28 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rotary_bwd_any
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * a.D; i += kThreads) {
+        const int which = i >= a.D;
         float s = 0.f;
         for (int w = 0; w < warps; ++w) s += s_dw[(int64_t)w * 2 * a.D + i];
-        a.dw_part[(int64_t)blockIdx.x * 2 * a.D + i] = s;
+        a.dw_part[((int64_t)which * gridDim.x + blockIdx.x) * a.D + (i - which * a.D)] = s;
     }
 }
 
-// Partial sums [blocks][2][D] -> the two weight gradients, in the weights' types.  A warp per value.
-__global__ void __launch_bounds__(kThreads) rotary_dw_kernel(const float* part, int blocks, int D, void* dwq, int qd, void* dwk, int kd) {
+// Partial sums, q_rows rows of D for the queries and k_rows for the keys, -> the two weight gradients in the weights' types.  A
+// warp per value.
+__global__ void __launch_bounds__(kThreads) rotary_dw_kernel(const float* part, int q_rows, int k_rows, int D, void* dwq, int qd, void* dwk, int kd) {
     const int i = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (i >= 2 * D) return;
-    void* out = i < D ? dwq : dwk;
+    const bool key = i >= D;
+    void* out = key ? dwk : dwq;
     if (!out) return;
+    const int at = key ? i - D : i, rows = key ? k_rows : q_rows;
+    const float* p = part + (key ? (int64_t)q_rows * D : 0) + at;
     float s = 0.f;
-    for (int b = lane; b < blocks; b += 32) s += part[(int64_t)b * 2 * D + i];
+    for (int b = lane; b < rows; b += 32) s += p[(int64_t)b * D];
     s = group_sum(s, 32);
     if (lane) return;
-    const int code = i < D ? qd : kd, at = i < D ? i : i - D;
+    const int code = key ? kd : qd;
     if (code == VTX_F32) static_cast<float*>(out)[at] = s;
     else if (code == VTX_BF16) static_cast<__nv_bfloat16*>(out)[at] = from_f32<__nv_bfloat16>(s);
     else static_cast<__half*>(out)[at] = from_f32<__half>(s);
@@ -510,15 +638,19 @@ int launch_fwd(const RotArgs& a, int64_t io, cudaStream_t s, const char* who) {
         VTX_DISPATCH_IO(io, T, rotary_fwd_any_kernel<T><<<(unsigned)blocks, kThreads, 0, s>>>(a));
         return check_launch(who);
     }
-    // one token per block until the blocks fill the machine several times over, then up to four
-    int tb = tokens >= (int64_t)kNumSMs * 32 ? 4 : 1;
-    tb = tb < (kThreads >> shift) ? tb : (kThreads >> shift);
-    const int64_t blocks = ceil_div<int64_t>(tokens, tb);
-    VTX_REQUIRE(blocks < ((int64_t)1 << 31), VTX_ERR_UNSUPPORTED, "%s: more than 2^31 tokens", who);
-    const size_t smem = (size_t)tb * (a.rot / 2) * sizeof(float2);
+    // up to eight steps a warp once that still gives every SM its warps; below, fewer, down to one
+    const int step = 32 >> shift;
+    int steps = 8;
+    auto chunks = [&](int h) { return (int)ceil_div<int64_t>(h, steps * step); };
+    auto per_token = [&] { return (int64_t)chunks(a.r[0].H) + chunks(a.r[1].H) + chunks(a.r[2].H); };
+    while (steps > 1 && tokens * per_token() < (int64_t)kNumSMs * kFwdBlocks * (kThreads / 32)) steps /= 2;
+    const Chunks ch{steps * step, chunks(a.r[0].H), chunks(a.r[1].H), chunks(a.r[2].H)};
+    const int64_t items = tokens * per_token(), blocks = ceil_div<int64_t>(items, kThreads / 32);
+    VTX_REQUIRE(items < ((int64_t)1 << 32) - kThreads, VTX_ERR_UNSUPPORTED, "%s: more than 2^32 pieces of heads", who);
+    const size_t smem = (size_t)(kThreads / 32) * a.rot * sizeof(float);
     VTX_DISPATCH_IO(io, T, {
-        if (a.inter) rotary_fwd_kernel<T, true><<<(unsigned)blocks, kThreads, smem, s>>>(a, tb, shift);
-        else rotary_fwd_kernel<T, false><<<(unsigned)blocks, kThreads, smem, s>>>(a, tb, shift);
+        if (a.inter) rotary_fwd_kernel<T, true><<<(unsigned)blocks, kThreads, smem, s>>>(a, ch, shift);
+        else rotary_fwd_kernel<T, false><<<(unsigned)blocks, kThreads, smem, s>>>(a, ch, shift);
     });
     return check_launch(who);
 }
@@ -531,6 +663,8 @@ int fill(RotArgs& a, const vtx_rotary_params& p, const char* who) {
     VTX_REQUIRE(p.rot >= 0 && p.rot % 2 == 0 && p.rot <= p.D, VTX_ERR_BAD_ARG, "%s: %lld rotated of %lld values of a head", who,
                 (long long)p.rot, (long long)p.D);
     const bool any = p.B > 0 && p.L > 0;
+    VTX_REQUIRE(!any || (p.B < ((int64_t)1 << 31) && p.L < ((int64_t)1 << 31) && p.B * p.L < ((int64_t)1 << 31)), VTX_ERR_UNSUPPORTED,
+                "%s: more than 2^31 tokens", who);
     VTX_REQUIRE(!any || !p.Hq || p.q, VTX_ERR_BAD_ARG, "%s: null pointer", who);
     VTX_REQUIRE(!any || !p.Hk || p.k, VTX_ERR_BAD_ARG, "%s: null pointer", who);
     VTX_REQUIRE(!any || (p.positions && (p.inv_freq || !p.rot)), VTX_ERR_BAD_ARG, "%s: null pointer", who);
@@ -586,32 +720,36 @@ extern "C" int vtx_qk_norm_rotary_bwd(const vtx_rotary_bwd_params* p, void* stre
     a.dy[0] = p->dq_out; a.dyb[0] = p->dq_out_stride_b; a.dyl[0] = p->dq_out_stride_l; a.dyh[0] = p->dq_out_stride_h;
     a.dy[1] = p->dk_out; a.dyb[1] = p->dk_out_stride_b; a.dyl[1] = p->dk_out_stride_l; a.dyh[1] = p->dk_out_stride_h;
     a.dw_part = static_cast<float*>(p->scratch);
-    int64_t blocks = 0;
+    int64_t q_rows = 0, k_rows = 0;
     long long launches = 1;
     if (tokens && f.Hq + f.Hk) {
         const int shift = vector_lanes(a, dtype_size(f.io_dtype));
         launches = 2;
         if (shift < 0) {
-            blocks = ceil_div<int64_t>(tokens * (f.Hq + f.Hk), kThreads / 32);
-            blocks = blocks < kBwdBlocks ? blocks : kBwdBlocks;
+            const int64_t warps = ceil_div<int64_t>(tokens * (f.Hq + f.Hk), kThreads / 32);
+            q_rows = k_rows = warps < kBwdBlocks ? warps : kBwdBlocks;
             VTX_DISPATCH_IO(f.io_dtype, T,
-                            rotary_bwd_any_kernel<T><<<(unsigned)blocks, kThreads, (size_t)(kThreads / 32) * 2 * f.D * 4, s>>>(a));
+                            rotary_bwd_any_kernel<T><<<(unsigned)q_rows, kThreads, (size_t)(kThreads / 32) * 2 * f.D * 4, s>>>(a));
         } else {
-            const int rows = kThreads >> shift;
-            const int tb = rows < 4 ? rows : 4;
-            blocks = ceil_div<int64_t>(tokens, tb);
-            blocks = blocks < kBwdBlocks ? blocks : kBwdBlocks;
-            size_t smem = (size_t)tb * (a.rot / 2) * sizeof(float2);
-            const size_t sums = (size_t)rows * f.D * 4;
+            // blocks for queries and keys in proportion to their heads, a warp at least a token
+            const int64_t most = ceil_div<int64_t>(tokens, kThreads / 32), total = kNumSMs * kBwdPerSM;
+            q_rows = f.Hq ? (total * f.Hq + (f.Hq + f.Hk) / 2) / (f.Hq + f.Hk) : 0;
+            if (f.Hq) q_rows = q_rows < 1 ? 1 : f.Hk && q_rows > total - 1 ? total - 1 : q_rows;
+            k_rows = f.Hk ? total - q_rows : 0;
+            q_rows = q_rows < most ? q_rows : most;
+            k_rows = k_rows < most ? k_rows : most;
+            size_t smem = (size_t)(kThreads / 32) * a.rot * sizeof(float);
+            const size_t sums = (size_t)(kThreads >> shift) * f.D * 4;
             smem = smem > sums ? smem : sums;
+            const unsigned blocks = (unsigned)(q_rows + k_rows);
             VTX_DISPATCH_IO(f.io_dtype, T, {
-                if (a.inter) rotary_bwd_kernel<T, true><<<(unsigned)blocks, kThreads, smem, s>>>(a, tb, shift);
-                else rotary_bwd_kernel<T, false><<<(unsigned)blocks, kThreads, smem, s>>>(a, tb, shift);
+                if (a.inter) rotary_bwd_kernel<T, true><<<blocks, kThreads, smem, s>>>(a, (int)q_rows, shift);
+                else rotary_bwd_kernel<T, false><<<blocks, kThreads, smem, s>>>(a, (int)q_rows, shift);
             });
         }
     }
     rotary_dw_kernel<<<(unsigned)ceil_div<int64_t>(2 * f.D, kThreads / 32), kThreads, 0, s>>>(
-        a.dw_part, (int)blocks, (int)f.D, f.q_weight ? p->dq_weight : nullptr, (int)f.q_weight_dtype,
+        a.dw_part, (int)q_rows, (int)k_rows, (int)f.D, f.q_weight ? p->dq_weight : nullptr, (int)f.q_weight_dtype,
         f.k_weight ? p->dk_weight : nullptr, (int)f.k_weight_dtype);
     return check_launch("qk_norm_rotary_bwd", launches);
 }
