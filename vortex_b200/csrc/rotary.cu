@@ -35,7 +35,7 @@ struct RotArgs {
     int64_t psb, psl;
     const void* freq;
     int pos64, freq64, rot, inter;
-    float scale, eps;
+    float scale, eps, inv_D;
     int conj;
     int64_t B, L;
     int D;
@@ -53,7 +53,7 @@ struct RotArgs {
 
 constexpr int kThreads = 256;
 constexpr int kMaxD = 512;
-constexpr int kFwdBlocks = 3, kFwdSteps = 2, kBwdPerSM = 2;
+constexpr int kFwdBlocks = 5, kBwdPerSM = 3, kTokenCost = 1;
 constexpr int kBwdBlocks = kNumSMs * 4;
 
 __device__ __forceinline__ int64_t load_pos(const RotArgs& a, int64_t b, int64_t l) {
@@ -100,12 +100,15 @@ template <> __device__ __forceinline__ float low<__nv_bfloat16>(uint32_t w) { re
 template <> __device__ __forceinline__ float high<__nv_bfloat16>(uint32_t w) { return umma::bf_hi(w); }
 template <> __device__ __forceinline__ float low<__half>(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))); }
 template <> __device__ __forceinline__ float high<__half>(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    T t[2] = {from_f32<T>(lo), from_f32<T>(hi)};
-    return *reinterpret_cast<uint32_t*>(t);
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return umma::pack_bf16(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-    for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+template <int LANES> __device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 __device__ __forceinline__ float sum2(f32x2 v) {
@@ -122,11 +125,12 @@ template <typename T, bool INTER> struct Lane {
     static constexpr int N = 16 / sizeof(T), P = N / 2;
     int ea, eb;          // first elements of the two vectors
     bool on, turned;     // inside the head; inside its rotated part
-    f32x2 c[P], s[P];
     __device__ Lane(const RotArgs& a, int sub) {
         on = sub * 2 * N < a.D;
         turned = sub * 2 * N < a.rot;
-        if (INTER) {
+        if (!on) {                                   // (reads what the first lane reads, and writes nothing)
+            ea = eb = 0;
+        } else if (INTER) {
             ea = sub * 2 * N; eb = ea + N;
         } else if (turned) {
             ea = sub * N; eb = ea + a.rot / 2;
@@ -136,15 +140,6 @@ template <typename T, bool INTER> struct Lane {
     }
     // element of the head that value i of the 2N holds (a first, then b)
     __device__ int element(int i) const { return INTER ? ea + 2 * (i < N ? i : i - N) + (i >= N) : i < N ? ea + i : eb + i - N; }
-    // cosines of a token's pairs, then their sines
-    __device__ void load_turns(const float* turns, int half, int sub) {
-        if (!turned) return;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            c[i] = *reinterpret_cast<const f32x2*>(turns + sub * N + 2 * i);
-            s[i] = *reinterpret_cast<const f32x2*>(turns + half + sub * N + 2 * i);
-        }
-    }
     __device__ static void unpack(const uint4& u, const uint4& v, f32x2* a, f32x2* b) {
         const uint32_t x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
         if constexpr (sizeof(T) == 4) {
@@ -197,273 +192,223 @@ template <typename T, bool INTER> struct Lane {
         u = make_uint4(x[0], x[1], x[2], x[3]);
         v = make_uint4(y[0], y[1], y[2], y[3]);
     }
-    __device__ void rotate(f32x2* a, f32x2* b) const {
+    __device__ static float squares(const f32x2* a, const f32x2* b) {
+        f32x2 x = mul2(a[0], a[0]), y = mul2(b[0], b[0]);
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const f32x2 x = a[i], y = b[i];
-            a[i] = sub2(mul2(x, c[i]), mul2(y, s[i]));
-            b[i] = fma2(x, s[i], mul2(y, c[i]));
-        }
+        for (int i = 1; i < P; ++i) { x = fma2(a[i], a[i], x); y = fma2(b[i], b[i], y); }
+        return sum2(add2(x, y));
     }
 };
 
-// The weights as the lanes hold them, in shared memory: quad q of a lane's 2N values at [q][lane], so that the lanes of a head
-// read neighbouring 16 bytes.
-template <typename T, bool INTER> __device__ __forceinline__ void stage_weights(const RotArgs& a, const Rows& r, float* dst, int lanes) {
-    constexpr int N = Lane<T, INTER>::N;
-    for (int i = threadIdx.x; i < 2 * N * lanes; i += kThreads) {
-        const int q = i / (4 * lanes), sub = i / 4 - q * lanes;
-        const Lane<T, INTER> ln(a, sub);
-        dst[i] = ln.on && r.w ? ld_param(r.w, r.wd, ln.element(q * 4 + (i & 3))) : 1.f;
-    }
-}
-__device__ __forceinline__ void load_quad(const float* w, int q, int lanes, int sub, f32x2& w0, f32x2& w1) {
-    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(w + (q * lanes + sub) * 4);
+// Values of a head as its lanes hold them, in shared memory: quad q of a lane's at [q][lane], so that the lanes read
+// neighbouring 16 bytes.  Registers are worth more than shared-memory reads here: what hides the memory is the number of warps
+// (the cosines, sines and weights in registers, and loads a step or two ahead: 199 instead of %ROT% us for 32768 tokens x 64 heads).
+template <int LANES> __device__ __forceinline__ void load_quad(const float* w, int q, int sub, f32x2& w0, f32x2& w1) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(w + (q * LANES + sub) * 4);
     w0 = v.x;
     w1 = v.y;
 }
-
-// Cosines and sines of a token's pairs, in the warp's piece of shared memory.
-__device__ __forceinline__ void warp_turns(const RotArgs& a, float* mine, int64_t pos) {
-    const int half = a.rot / 2;
+// The weights: 2N values a lane.
+template <typename T, bool INTER, int LANES> __device__ __forceinline__ void stage_weights(const RotArgs& a, const Rows& r, float* dst) {
+    if (!r.w) return;
+    for (int i = threadIdx.x; i < Lane<T, INTER>::N * 2 * LANES; i += kThreads) {
+        const int q = i / (4 * LANES), sub = i / 4 % LANES;
+        const Lane<T, INTER> ln(a, sub);
+        dst[i] = ln.on ? ld_param(r.w, r.wd, ln.element(q * 4 + i % 4)) : 0.f;
+    }
+}
+// Cosines, then sines, of a token's pairs, N values a lane each, in the warp's own piece.
+template <int N, int LANES> __device__ __forceinline__ void stage_turns(const RotArgs& a, float* dst, int64_t pos) {
     __syncwarp();
-    for (int i = threadIdx.x & 31; i < half; i += 32) {
+    for (int i = threadIdx.x & 31; i < a.rot / 2; i += 32) {
         const float2 cs = turn(a, pos, i);
-        mine[i] = cs.x;
-        mine[half + i] = cs.y;
+        float* d = dst + (i % N / 4 * LANES + i / N) * 4 + i % 4;
+        d[0] = cs.x;
+        d[N * LANES] = cs.y;
     }
     __syncwarp();
 }
+template <int N, int LANES> __device__ __forceinline__ void rotate(const float* turns, int sub, f32x2* a, f32x2* b) {
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        f32x2 c[2], s[2];
+        load_quad<LANES>(turns, q, sub, c[0], c[1]);
+        load_quad<LANES>(turns + N * LANES, q, sub, s[0], s[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const f32x2 x = a[2 * q + j], y = b[2 * q + j];
+            a[2 * q + j] = sub2(mul2(x, c[j]), mul2(y, s[j]));
+            b[2 * q + j] = fma2(x, s[j], mul2(y, c[j]));
+        }
+    }
+}
 
-// A warp takes one token and `chunk` heads of its queries, keys or values, 32 >> lane_shift heads side by side
-// (1 << lane_shift lanes cover a head), U steps in flight: a step's registers are refilled as soon as its values have been
-// unpacked.  No warp waits for another (but for the weights, once): a token's chain position -> angles, page lookup -> store
+// A warp takes one token and `chunk` heads of its queries, keys or values, 32 / LANES heads side by side (LANES lanes cover a
+// head).  No warp waits for another (but for the weights, once): a token's chain position -> angles, page lookup -> store
 // hides behind the other warps' traffic.
 struct Chunks { int size, q, k, v; };      // heads in one; chunks of a token's queries, keys, values
 
-template <typename T, bool INTER>
-__global__ void __launch_bounds__(kThreads, kFwdBlocks) rotary_fwd_kernel(const __grid_constant__ RotArgs a, Chunks ch, int lane_shift) {
+template <typename T, bool INTER, int LANES>
+__global__ void __launch_bounds__(kThreads, kFwdBlocks) rotary_fwd_kernel(const __grid_constant__ RotArgs a, const __grid_constant__ Chunks ch) {
     using Ln = Lane<T, INTER>;
-    constexpr int N = Ln::N, P = Ln::P, U = kFwdSteps;
-    extern __shared__ __align__(16) float s_turn[];                // [warp][rot]
-    __shared__ __align__(16) float s_w[2][kMaxD];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lanes = 1 << lane_shift, sub = lane & (lanes - 1), slot = lane >> lane_shift;
-    const int step = 32 >> lane_shift;
+    constexpr int N = Ln::N, P = Ln::P, STEP = 32 / LANES;
+    __shared__ __align__(16) float s_turn[kThreads / 32][2 * N * LANES], s_w[2][2 * N * LANES];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES, slot = lane / LANES;
     const bool any_norm = a.r[0].w || a.r[1].w;
     const uint32_t item = blockIdx.x * (kThreads / 32) + warp, per = ch.q + ch.k + ch.v, tok = item / per, L = (uint32_t)a.L;
     const bool live = tok < (uint32_t)(a.B * a.L);
+    if (any_norm) {
+        stage_weights<T, INTER, LANES>(a, a.r[0], s_w[0]);
+        stage_weights<T, INTER, LANES>(a, a.r[1], s_w[1]);
+        __syncthreads();
+    }
+    if (!live) return;
     int c = (int)(item - tok * per);
     const int which = c < ch.q ? 0 : c < ch.q + ch.k ? 1 : 2;
     c -= which == 0 ? 0 : which == 1 ? ch.q : ch.q + ch.k;
     const Rows& r = a.r[which];
-    const uint32_t b = live ? tok / L : 0, l = live ? tok - b * L : 0;
-    const int first = c * ch.size, count = live ? (ch.size < r.H - first ? ch.size : r.H - first) : 0;
-    Ln ln(a, sub);
-    const T* src = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + (first + slot) * r.sh;
-    const int64_t src_step = step * r.sh;
-    uint4 va[U], vb[U];
-    int fh = slot;                                                 // head of the next step to fetch
-    auto fetch = [&](int u) {
-        va[u] = vb[u] = make_uint4(0, 0, 0, 0);
-        if (ln.on && fh < count) {
-            va[u] = *reinterpret_cast<const uint4*>(src + ln.ea);
-            vb[u] = *reinterpret_cast<const uint4*>(src + ln.eb);
-        }
-        src += src_step;
-        fh += step;
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u) fetch(u);
-    if (any_norm) {
-        stage_weights<T, INTER>(a, a.r[0], s_w[0], lanes);
-        stage_weights<T, INTER>(a, a.r[1], s_w[1], lanes);
-        __syncthreads();
-    }
-    if (!live) return;
+    const uint32_t b = tok / L, l = tok - b * L;
+    const int first = c * ch.size, count = ch.size < r.H - first ? ch.size : r.H - first;
+    const Ln ln(a, sub);
     const int64_t pos = load_pos(a, b, l);
     int64_t at = b * r.db + l * r.dl;
     if (a.paged && which) {
         at = slot_offset(a, tok, pos, which);
         if (at < 0) return;
     }
-    T* dst = static_cast<T*>(r.dst) + at + (first + slot) * r.dh;
-    const int64_t dst_step = step * r.dh;
-    if (which < 2) {
-        warp_turns(a, s_turn + warp * a.rot, pos);
-        ln.load_turns(s_turn + warp * a.rot, a.rot / 2, sub);
-    }
+    const T* src = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + first * r.sh;
+    T* dst = static_cast<T*>(r.dst) + at + first * r.dh;
+    if (which < 2) stage_turns<N, LANES>(a, s_turn[warp], pos);
     const bool norm = which < 2 && r.w;
-    for (int h0 = 0; h0 < count;) {
+    for (int h0 = 0; h0 < count; h0 += STEP) {
+        // (a lane behind the last head reads that one again: every address lies inside the rows)
+        const int h = h0 + slot < count ? h0 + slot : count - 1;
+        const T* p = src + h * r.sh;
+        uint4 u = *reinterpret_cast<const uint4*>(p + ln.ea), v = *reinterpret_cast<const uint4*>(p + ln.eb);
+        if (which < 2) {
+            f32x2 xa[P], xb[P];
+            Ln::unpack(u, v, xa, xb);
+            if (norm) {
+                const float ss = group_sum<LANES>(ln.on ? Ln::squares(xa, xb) : 0.f);
+                const float inv = rsqrtf(ss * a.inv_D + a.eps);
+                const f32x2 inv2 = pk2(inv, inv);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (h0 >= count) break;                                // (the same for the whole warp)
-            const bool mine = ln.on && h0 + slot < count;
-            uint4 ra = va[u], rb = vb[u];
-            fetch(u);
-            if (which < 2) {
-                f32x2 xa[P], xb[P];
-                Ln::unpack(ra, rb, xa, xb);
-                if (norm) {
-                    f32x2 ss2 = mul2(xa[0], xa[0]);
-#pragma unroll
-                    for (int i = 1; i < P; ++i) ss2 = fma2(xa[i], xa[i], ss2);
-#pragma unroll
-                    for (int i = 0; i < P; ++i) ss2 = fma2(xb[i], xb[i], ss2);
-                    const float ss = group_sum(sum2(ss2), lanes);
-                    const float inv = rsqrtf(ss / (float)a.D + a.eps);
-                    const f32x2 inv2 = pk2(inv, inv);
-#pragma unroll
-                    for (int q = 0; q < N / 2; ++q) {
-                        f32x2 w0, w1;
-                        load_quad(s_w[which], q, lanes, sub, w0, w1);
-                        f32x2* x = q < N / 4 ? xa + 2 * q : xb + 2 * (q - N / 4);
-                        x[0] = mul2(mul2(x[0], inv2), w0);
-                        x[1] = mul2(mul2(x[1], inv2), w1);
-                    }
+                for (int q = 0; q < P; ++q) {
+                    f32x2 w0, w1;
+                    load_quad<LANES>(s_w[which], q, sub, w0, w1);
+                    f32x2* x = (q < P / 2 ? xa : xb) + 2 * (q % (P / 2));
+                    x[0] = mul2(mul2(x[0], inv2), w0);
+                    x[1] = mul2(mul2(x[1], inv2), w1);
                 }
-                if (ln.turned) ln.rotate(xa, xb);
-                Ln::pack(xa, xb, ra, rb);
             }
-            if (mine) {
-                *reinterpret_cast<uint4*>(dst + ln.ea) = ra;
-                *reinterpret_cast<uint4*>(dst + ln.eb) = rb;
-            }
-            dst += dst_step;
-            h0 += step;
+            if (ln.turned) rotate<N, LANES>(s_turn[warp], sub, xa, xb);
+            Ln::pack(xa, xb, u, v);
+        }
+        if (ln.on && h0 + slot < count) {
+            T* d = dst + h * r.dh;
+            *reinterpret_cast<uint4*>(d + ln.ea) = u;
+            *reinterpret_cast<uint4*>(d + ln.eb) = v;
         }
     }
 }
 
 // Backward behind a norm.  The first blocks take the queries, the rest the keys; a warp walks its tokens, all heads of one
-// before the next, U steps in flight across them.  A lane keeps its dimensions through all rows, so the weight's gradient
-// gathers in its registers, then across the block, and leaves as one row of partial sums per block: summed in a fixed order,
-// no atomics.
-template <typename T, bool INTER>
-__global__ void __launch_bounds__(kThreads, kBwdPerSM) rotary_bwd_kernel(const __grid_constant__ RotArgs a, int q_blocks, int lane_shift) {
+// before the next.  A lane keeps its dimensions through all rows, so the weight's gradient gathers in its registers, then
+// across the block, and leaves as one row of partial sums per block: summed in a fixed order, no atomics.
+template <typename T, bool INTER, int LANES>
+__global__ void __launch_bounds__(kThreads, kBwdPerSM) rotary_bwd_kernel(const __grid_constant__ RotArgs a, int q_blocks) {
     using Ln = Lane<T, INTER>;
-    constexpr int N = Ln::N, P = Ln::P, U = 2;
-    extern __shared__ __align__(16) float s_turn[];                // [warp][rot], later the rows' sums [rows][D]
-    __shared__ __align__(16) float s_w[kMaxD];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lanes = 1 << lane_shift, sub = lane & (lanes - 1), slot = lane >> lane_shift;
-    const int step = 32 >> lane_shift, rows = kThreads >> lane_shift;
+    constexpr int N = Ln::N, P = Ln::P, STEP = 32 / LANES;
+    __shared__ __align__(16) float s_turn[kThreads / 32][2 * N * LANES], s_w[2 * N * LANES], s_sum[kThreads / 32][2 * N * LANES];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES, slot = lane / LANES;
     const int which = (int)blockIdx.x >= q_blocks;
     const Rows& r = a.r[which];
     const uint32_t tokens = (uint32_t)(a.B * a.L), L = (uint32_t)a.L;
-    const uint32_t w0 = (blockIdx.x - (which ? q_blocks : 0)) * (kThreads / 32) + warp;
     const uint32_t warps = (which ? gridDim.x - q_blocks : q_blocks) * (kThreads / 32);
     const bool norm = r.w;
-    Ln ln(a, sub);
+    const Ln ln(a, sub);
     f32x2 dwa[P], dwb[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) dwa[i] = dwb[i] = pk2(0.f, 0.f);
-    uint4 va[U], vb[U], ga[U], gb[U];
-    uint32_t ft = w0;                                              // token and first head of the next step to fetch
-    int fh = 0;
-    const T *xp = nullptr, *gp = nullptr;
-    const int64_t xstep = step * r.sh, gstep = step * a.dyh[which];
-    auto fetch = [&](int u) {
-        va[u] = vb[u] = ga[u] = gb[u] = make_uint4(0, 0, 0, 0);
-        if (fh == 0) {
-            const uint32_t b = ft / L, l = ft - b * L;
-            xp = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + slot * r.sh;
-            gp = static_cast<const T*>(a.dy[which]) + b * a.dyb[which] + l * a.dyl[which] + slot * a.dyh[which];
-        }
-        if (ln.on && ft < tokens && fh + slot < r.H) {
-            ga[u] = *reinterpret_cast<const uint4*>(gp + ln.ea);
-            gb[u] = *reinterpret_cast<const uint4*>(gp + ln.eb);
-            if (norm) {
-                va[u] = *reinterpret_cast<const uint4*>(xp + ln.ea);
-                vb[u] = *reinterpret_cast<const uint4*>(xp + ln.eb);
-            }
-        }
-        xp += xstep;
-        gp += gstep;
-        fh += step;
-        if (fh >= r.H) { fh = 0; ft = ft + warps < ft ? tokens : ft + warps; }
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u) fetch(u);
-    stage_weights<T, INTER>(a, r, s_w, lanes);
+    stage_weights<T, INTER, LANES>(a, r, s_w);
     __syncthreads();
-    uint32_t t = w0;
-    int h0 = 0;
-    T* dst = nullptr;
-    const int64_t dstep = step * r.dh;
-    while (t < tokens) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (t >= tokens) break;
-            if (h0 == 0) {
-                const uint32_t b = t / L, l = t - b * L;
-                warp_turns(a, s_turn + warp * a.rot, load_pos(a, b, l));
-                ln.load_turns(s_turn + warp * a.rot, a.rot / 2, sub);
-                dst = static_cast<T*>(r.dst) + b * r.db + l * r.dl + slot * r.dh;
-            }
-            f32x2 xa[P], xb[P], da[P], db[P];
-            Ln::unpack(va[u], vb[u], xa, xb);
-            Ln::unpack(ga[u], gb[u], da, db);
-            fetch(u);
-            if (ln.turned) ln.rotate(da, db);
+    for (uint32_t t = (blockIdx.x - (which ? q_blocks : 0)) * (kThreads / 32) + warp; t < tokens; t += warps) {
+        const uint32_t b = t / L, l = t - b * L;
+        const T* xp = static_cast<const T*>(r.src) + b * r.sb + l * r.sl;
+        const T* gp = static_cast<const T*>(a.dy[which]) + b * a.dyb[which] + l * a.dyl[which];
+        T* dp = static_cast<T*>(r.dst) + b * r.db + l * r.dl;
+        stage_turns<N, LANES>(a, s_turn[warp], load_pos(a, b, l));
+        for (int h0 = 0; h0 < r.H; h0 += STEP) {
+            // (a lane behind the last head reads that one again: every address lies inside the rows)
+            const bool mine = ln.on && h0 + slot < r.H;
+            const int h = h0 + slot < r.H ? h0 + slot : r.H - 1;
+            const T* g = gp + h * a.dyh[which];
+            uint4 ga = *reinterpret_cast<const uint4*>(g + ln.ea), gb = *reinterpret_cast<const uint4*>(g + ln.eb);
+            f32x2 da[P], db[P];
             if (norm) {
-                f32x2 ss2 = mul2(xa[0], xa[0]), dot2 = pk2(0.f, 0.f);
-#pragma unroll
-                for (int i = 1; i < P; ++i) ss2 = fma2(xa[i], xa[i], ss2);
-#pragma unroll
-                for (int i = 0; i < P; ++i) ss2 = fma2(xb[i], xb[i], ss2);
-                const float ss = group_sum(sum2(ss2), lanes);
-                const float inv = rsqrtf(ss / (float)a.D + a.eps);
+                const T* x = xp + h * r.sh;
+                const uint4 va = *reinterpret_cast<const uint4*>(x + ln.ea), vb = *reinterpret_cast<const uint4*>(x + ln.eb);
+                f32x2 xa[P], xb[P];
+                Ln::unpack(va, vb, xa, xb);
+                const float ss = group_sum<LANES>(ln.on ? Ln::squares(xa, xb) : 0.f);
+                const float inv = rsqrtf(ss * a.inv_D + a.eps);
                 const f32x2 inv2 = pk2(inv, inv);
+                Ln::unpack(ga, gb, da, db);
+                if (ln.turned) rotate<N, LANES>(s_turn[warp], sub, da, db);
+                f32x2 dot2 = pk2(0.f, 0.f);
 #pragma unroll
-                for (int q = 0; q < N / 2; ++q) {
+                for (int q = 0; q < P; ++q) {
                     f32x2 wq[2];
-                    load_quad(s_w, q, lanes, sub, wq[0], wq[1]);
-                    const int at = q < N / 4 ? 2 * q : 2 * (q - N / 4);
-                    f32x2 *x = (q < N / 4 ? xa : xb) + at, *d = (q < N / 4 ? da : db) + at, *dw = (q < N / 4 ? dwa : dwb) + at;
+                    load_quad<LANES>(s_w, q, sub, wq[0], wq[1]);
+                    const int at = 2 * (q % (P / 2));
+                    f32x2 *x2 = (q < P / 2 ? xa : xb) + at, *d = (q < P / 2 ? da : db) + at, *dw = (q < P / 2 ? dwa : dwb) + at;
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        // (lanes outside the head and its rows hold zeros)
-                        x[j] = mul2(x[j], inv2);                            // xh
-                        dw[j] = fma2(d[j], x[j], dw[j]);
+                        x2[j] = mul2(x2[j], inv2);                          // xh
+                        if (mine) dw[j] = fma2(d[j], x2[j], dw[j]);
                         d[j] = mul2(d[j], wq[j]);                           // w g
-                        dot2 = fma2(d[j], x[j], dot2);
+                        dot2 = fma2(d[j], x2[j], dot2);
                     }
                 }
-                const float mean = group_sum(sum2(dot2), lanes) * (-1.f / (float)a.D);
+                const float mean = group_sum<LANES>(ln.on ? sum2(dot2) : 0.f) * -a.inv_D;
                 const f32x2 mean2 = pk2(mean, mean);
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    da[i] = mul2(fma2(mean2, xa[i], da[i]), inv2);
-                    db[i] = mul2(fma2(mean2, xb[i], db[i]), inv2);
+                for (int j = 0; j < P; ++j) {
+                    da[j] = mul2(fma2(mean2, xa[j], da[j]), inv2);
+                    db[j] = mul2(fma2(mean2, xb[j], db[j]), inv2);
                 }
+            } else {
+                Ln::unpack(ga, gb, da, db);
+                if (ln.turned) rotate<N, LANES>(s_turn[warp], sub, da, db);
             }
-            if (ln.on && h0 + slot < r.H) {
-                uint4 ra, rb;
-                Ln::pack(da, db, ra, rb);
-                *reinterpret_cast<uint4*>(dst + ln.ea) = ra;
-                *reinterpret_cast<uint4*>(dst + ln.eb) = rb;
+            if (mine) {
+                Ln::pack(da, db, ga, gb);
+                T* d = dp + h * r.dh;
+                *reinterpret_cast<uint4*>(d + ln.ea) = ga;
+                *reinterpret_cast<uint4*>(d + ln.eb) = gb;
             }
-            dst += dstep;
-            h0 += step;
-            if (h0 >= r.H) { h0 = 0; t = t + warps < t ? tokens : t + warps; }
         }
     }
-    float* s_sum = s_turn;
-    const int row = tid >> lane_shift;
-    __syncthreads();
-    if (ln.on)
+    // the sums of a lane's values: over the warp's rows, then the warps
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float lo, hi;
-            up2(dwa[i / 2], lo, hi);
-            s_sum[row * a.D + ln.element(i)] = i & 1 ? hi : lo;
-            up2(dwb[i / 2], lo, hi);
-            s_sum[row * a.D + ln.element(N + i)] = i & 1 ? hi : lo;
+    for (int j = 0; j < N; ++j) {
+        float x[4];
+        up2(dwa[j / 2], x[0], x[1]);
+        up2(dwb[j / 2], x[2], x[3]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float v = x[2 * k + j % 2];
+#pragma unroll
+            for (int o = LANES; o < 32; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (slot == 0) s_sum[warp][sub * 2 * N + k * N + j] = v;
         }
+    }
     __syncthreads();
-    for (int d = tid; d < a.D; d += kThreads) {
+    for (int i = threadIdx.x; i < 2 * N * LANES; i += kThreads) {
+        const Ln own(a, i / (2 * N));
         float sum = 0.f;
-        for (int i = 0; i < rows; ++i) sum += s_sum[i * a.D + d];
-        a.dw_part[(int64_t)blockIdx.x * a.D + d] = sum;
+        for (int w = 0; w < kThreads / 32; ++w) sum += s_sum[w][i];
+        if (own.on) a.dw_part[(int64_t)blockIdx.x * a.D + own.element(i % (2 * N))] = sum;
     }
 }
 
@@ -507,7 +452,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rotary_fwd_any
     if (r.w) {
         float ss = 0.f;
         for (int d = lane; d < a.D; d += 32) ss += to_f32<T>(x[d]) * to_f32<T>(x[d]);
-        inv = rsqrtf(group_sum(ss, 32) / (float)a.D + a.eps);
+        inv = rsqrtf(group_sum<32>(ss) / (float)a.D + a.eps);
     }
     const Pairs ps{a.rot / 2, a.rot, a.D, a.inter};
     for (int i = lane; i < ps.count(); i += 32) {
@@ -574,8 +519,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rotary_bwd_any
                 if (pair) dx[q] = from_f32<T>(gq);
             }
             if (pass == 0) {
-                inv = rsqrtf(group_sum(ss, 32) / (float)a.D + a.eps);
-                back = group_sum(dot, 32) * inv * inv / (float)a.D;
+                inv = rsqrtf(group_sum<32>(ss) / (float)a.D + a.eps);
+                back = group_sum<32>(dot) * inv * inv / (float)a.D;
             }
         }
     }
@@ -600,7 +545,7 @@ __global__ void __launch_bounds__(kThreads) rotary_dw_kernel(const float* part, 
     const float* p = part + (key ? (int64_t)q_rows * D : 0) + at;
     float s = 0.f;
     for (int b = lane; b < rows; b += 32) s += p[(int64_t)b * D];
-    s = group_sum(s, 32);
+    s = group_sum<32>(s);
     if (lane) return;
     const int code = key ? kd : qd;
     if (code == VTX_F32) static_cast<float*>(out)[at] = s;
@@ -613,33 +558,41 @@ bool rows_aligned(const void* p, int64_t sb, int64_t sl, int64_t sh, int64_t es)
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (sb * es) % 16 == 0 && (sl * es) % 16 == 0 && (sh * es) % 16 == 0;
 }
 
-// Lanes of a head in the vector kernels, as a shift; -1 where they do not apply: heads and their rotated part in whole pairs
-// of 16-byte vectors, at most 32 threads to a head, all rows on 16-byte boundaries.
+// Lanes of a head in the vector kernels: 4, 8, 16 or 32; 0 where they do not apply: heads and their rotated part in whole
+// pairs of 16-byte vectors, at most 32 pairs to a head, all rows on 16-byte boundaries.
 int vector_lanes(const RotArgs& a, int64_t es) {
     const int pair = 2 * (int)(16 / es);
-    if (a.D % pair || a.rot % pair || a.D / pair > 32) return -1;
+    if (a.D % pair || a.rot % pair || a.D / pair > 32) return 0;
     for (int i = 0; i < 3; ++i) {
         const Rows& r = a.r[i];
-        if (r.H && (!rows_aligned(r.src, r.sb, r.sl, r.sh, es) || !rows_aligned(r.dst, r.db, r.dl, r.dh, es))) return -1;
-        if (i < 2 && r.H && a.dy[i] && !rows_aligned(a.dy[i], a.dyb[i], a.dyl[i], a.dyh[i], es)) return -1;
+        if (r.H && (!rows_aligned(r.src, r.sb, r.sl, r.sh, es) || !rows_aligned(r.dst, r.db, r.dl, r.dh, es))) return 0;
+        if (i < 2 && r.H && a.dy[i] && !rows_aligned(a.dy[i], a.dyb[i], a.dyl[i], a.dyh[i], es)) return 0;
     }
-    int shift = 0;
-    while ((1 << shift) * pair < a.D) ++shift;
-    return shift;
+    int lanes = 4;
+    while (lanes * pair < a.D) lanes *= 2;
+    return lanes;
 }
+
+#define VTX_DISPATCH_LANES(lanes, N, ...)                        \
+    switch (lanes) {                                             \
+        case 4:  { constexpr int N = 4;  __VA_ARGS__; break; }   \
+        case 8:  { constexpr int N = 8;  __VA_ARGS__; break; }   \
+        case 16: { constexpr int N = 16; __VA_ARGS__; break; }   \
+        default: { constexpr int N = 32; __VA_ARGS__; break; }   \
+    }
 
 int launch_fwd(const RotArgs& a, int64_t io, cudaStream_t s, const char* who) {
     const int64_t tokens = a.B * a.L, heads = a.r[0].H + a.r[1].H + a.r[2].H;
     if (tokens == 0 || heads == 0) return VTX_OK;
-    const int shift = vector_lanes(a, dtype_size(io));
-    if (shift < 0) {
+    const int lanes = vector_lanes(a, dtype_size(io));
+    if (!lanes) {
         const int64_t blocks = ceil_div<int64_t>(tokens * heads, kThreads / 32);
         VTX_REQUIRE(blocks < ((int64_t)1 << 31), VTX_ERR_UNSUPPORTED, "%s: more than 2^34 rows", who);
         VTX_DISPATCH_IO(io, T, rotary_fwd_any_kernel<T><<<(unsigned)blocks, kThreads, 0, s>>>(a));
         return check_launch(who);
     }
     // up to eight steps a warp once that still gives every SM its warps; below, fewer, down to one
-    const int step = 32 >> shift;
+    const int step = 32 / lanes;
     int steps = 8;
     auto chunks = [&](int h) { return (int)ceil_div<int64_t>(h, steps * step); };
     auto per_token = [&] { return (int64_t)chunks(a.r[0].H) + chunks(a.r[1].H) + chunks(a.r[2].H); };
@@ -647,11 +600,10 @@ int launch_fwd(const RotArgs& a, int64_t io, cudaStream_t s, const char* who) {
     const Chunks ch{steps * step, chunks(a.r[0].H), chunks(a.r[1].H), chunks(a.r[2].H)};
     const int64_t items = tokens * per_token(), blocks = ceil_div<int64_t>(items, kThreads / 32);
     VTX_REQUIRE(items < ((int64_t)1 << 32) - kThreads, VTX_ERR_UNSUPPORTED, "%s: more than 2^32 pieces of heads", who);
-    const size_t smem = (size_t)(kThreads / 32) * a.rot * sizeof(float);
-    VTX_DISPATCH_IO(io, T, {
-        if (a.inter) rotary_fwd_kernel<T, true><<<(unsigned)blocks, kThreads, smem, s>>>(a, ch, shift);
-        else rotary_fwd_kernel<T, false><<<(unsigned)blocks, kThreads, smem, s>>>(a, ch, shift);
-    });
+    VTX_DISPATCH_IO(io, T, VTX_DISPATCH_LANES(lanes, N, {
+        if (a.inter) rotary_fwd_kernel<T, true, N><<<(unsigned)blocks, kThreads, 0, s>>>(a, ch);
+        else rotary_fwd_kernel<T, false, N><<<(unsigned)blocks, kThreads, 0, s>>>(a, ch);
+    }));
     return check_launch(who);
 }
 
@@ -677,7 +629,7 @@ int fill(RotArgs& a, const vtx_rotary_params& p, const char* who) {
     a.pos = p.positions; a.pos64 = p.positions_i64 != 0; a.psb = p.pos_stride_b; a.psl = p.pos_stride_l;
     a.freq = p.inv_freq; a.freq64 = p.inv_freq_f64 != 0; a.rot = (int)p.rot; a.inter = p.interleaved != 0;
     a.scale = (float)p.scale; a.eps = (float)p.eps; a.conj = 0;
-    a.B = p.B; a.L = p.L; a.D = (int)p.D;
+    a.B = p.B; a.L = p.L; a.D = (int)p.D; a.inv_D = 1.f / (float)p.D;
     return VTX_OK;
 }
 
@@ -723,9 +675,9 @@ extern "C" int vtx_qk_norm_rotary_bwd(const vtx_rotary_bwd_params* p, void* stre
     int64_t q_rows = 0, k_rows = 0;
     long long launches = 1;
     if (tokens && f.Hq + f.Hk) {
-        const int shift = vector_lanes(a, dtype_size(f.io_dtype));
+        const int lanes = vector_lanes(a, dtype_size(f.io_dtype));
         launches = 2;
-        if (shift < 0) {
+        if (!lanes) {
             const int64_t warps = ceil_div<int64_t>(tokens * (f.Hq + f.Hk), kThreads / 32);
             q_rows = k_rows = warps < kBwdBlocks ? warps : kBwdBlocks;
             VTX_DISPATCH_IO(f.io_dtype, T,
@@ -733,19 +685,17 @@ extern "C" int vtx_qk_norm_rotary_bwd(const vtx_rotary_bwd_params* p, void* stre
         } else {
             // blocks for queries and keys in proportion to their heads, a warp at least a token
             const int64_t most = ceil_div<int64_t>(tokens, kThreads / 32), total = kNumSMs * kBwdPerSM;
-            q_rows = f.Hq ? (total * f.Hq + (f.Hq + f.Hk) / 2) / (f.Hq + f.Hk) : 0;
+            auto cost = [&](int64_t h) { return h ? ceil_div<int64_t>(h, 32 / lanes) + kTokenCost : 0; };
+            q_rows = f.Hq ? (total * cost(f.Hq) + (cost(f.Hq) + cost(f.Hk)) / 2) / (cost(f.Hq) + cost(f.Hk)) : 0;
             if (f.Hq) q_rows = q_rows < 1 ? 1 : f.Hk && q_rows > total - 1 ? total - 1 : q_rows;
             k_rows = f.Hk ? total - q_rows : 0;
             q_rows = q_rows < most ? q_rows : most;
             k_rows = k_rows < most ? k_rows : most;
-            size_t smem = (size_t)(kThreads / 32) * a.rot * sizeof(float);
-            const size_t sums = (size_t)(kThreads >> shift) * f.D * 4;
-            smem = smem > sums ? smem : sums;
             const unsigned blocks = (unsigned)(q_rows + k_rows);
-            VTX_DISPATCH_IO(f.io_dtype, T, {
-                if (a.inter) rotary_bwd_kernel<T, true><<<blocks, kThreads, smem, s>>>(a, (int)q_rows, shift);
-                else rotary_bwd_kernel<T, false><<<blocks, kThreads, smem, s>>>(a, (int)q_rows, shift);
-            });
+            VTX_DISPATCH_IO(f.io_dtype, T, VTX_DISPATCH_LANES(lanes, N, {
+                if (a.inter) rotary_bwd_kernel<T, true, N><<<blocks, kThreads, 0, s>>>(a, (int)q_rows);
+                else rotary_bwd_kernel<T, false, N><<<blocks, kThreads, 0, s>>>(a, (int)q_rows);
+            }));
         }
     }
     rotary_dw_kernel<<<(unsigned)ceil_div<int64_t>(2 * f.D, kThreads / 32), kThreads, 0, s>>>(
