@@ -125,11 +125,12 @@ template <typename T, bool INTER> struct Lane {
     static constexpr int N = 16 / sizeof(T), P = N / 2;
     int ea, eb;          // first elements of the two vectors
     bool on, turned;     // inside the head; inside its rotated part
+    __device__ int apart() const { return INTER ? N : eb - ea; }
     __device__ Lane(const RotArgs& a, int sub) {
         on = sub * 2 * N < a.D;
         turned = sub * 2 * N < a.rot;
         if (!on) {                                   // (reads what the first lane reads, and writes nothing)
-            ea = eb = 0;
+            ea = 0; eb = INTER ? N : 0;
         } else if (INTER) {
             ea = sub * 2 * N; eb = ea + N;
         } else if (turned) {
@@ -257,34 +258,44 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks) rotary_fwd_kernel(const 
     const bool any_norm = a.r[0].w || a.r[1].w;
     const uint32_t item = blockIdx.x * (kThreads / 32) + warp, per = ch.q + ch.k + ch.v, tok = item / per, L = (uint32_t)a.L;
     const bool live = tok < (uint32_t)(a.B * a.L);
+    int c = (int)(item - tok * per);
+    const int which = c < ch.q ? 0 : c < ch.q + ch.k ? 1 : 2;
+    c -= which == 0 ? 0 : which == 1 ? ch.q : ch.q + ch.k;
+    const Rows& r = a.r[which];
+    const uint32_t b = live ? tok / L : 0, l = live ? tok - b * L : 0;     // (a warp behind the last token reads the first)
+    const int first = c * ch.size, count = ch.size < r.H - first ? ch.size : r.H - first;
+    const Ln ln(a, sub);
+    const int apart = ln.apart();
+    const T* const head0 = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + first * r.sh + ln.ea;
+    const T* src = head0 + slot * r.sh;
+    const int64_t src_step = STEP * r.sh, dst_step = STEP * r.dh;
+    uint4 nu, nv;                                                  // loaded a step ahead
+    // (a lane behind the last head reads the first: every address lies inside the rows)
+    auto fetch = [&](int h0) {
+        const T* p = h0 + STEP > count && h0 + slot >= count ? head0 : src;
+        nu = *reinterpret_cast<const uint4*>(p);
+        nv = *reinterpret_cast<const uint4*>(p + apart);
+        src += src_step;
+    };
+    fetch(0);
     if (any_norm) {
         stage_weights<T, INTER, LANES>(a, a.r[0], s_w[0]);
         stage_weights<T, INTER, LANES>(a, a.r[1], s_w[1]);
         __syncthreads();
     }
     if (!live) return;
-    int c = (int)(item - tok * per);
-    const int which = c < ch.q ? 0 : c < ch.q + ch.k ? 1 : 2;
-    c -= which == 0 ? 0 : which == 1 ? ch.q : ch.q + ch.k;
-    const Rows& r = a.r[which];
-    const uint32_t b = tok / L, l = tok - b * L;
-    const int first = c * ch.size, count = ch.size < r.H - first ? ch.size : r.H - first;
-    const Ln ln(a, sub);
     const int64_t pos = load_pos(a, b, l);
     int64_t at = b * r.db + l * r.dl;
     if (a.paged && which) {
         at = slot_offset(a, tok, pos, which);
         if (at < 0) return;
     }
-    const T* src = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + first * r.sh;
-    T* dst = static_cast<T*>(r.dst) + at + first * r.dh;
+    T* dst = static_cast<T*>(r.dst) + at + (first + slot) * r.dh + ln.ea;
     if (which < 2) stage_turns<N, LANES>(a, s_turn[warp], pos);
     const bool norm = which < 2 && r.w;
     for (int h0 = 0; h0 < count; h0 += STEP) {
-        // (a lane behind the last head reads that one again: every address lies inside the rows)
-        const int h = h0 + slot < count ? h0 + slot : count - 1;
-        const T* p = src + h * r.sh;
-        uint4 u = *reinterpret_cast<const uint4*>(p + ln.ea), v = *reinterpret_cast<const uint4*>(p + ln.eb);
+        uint4 u = nu, v = nv;
+        if (h0 + STEP < count) fetch(h0 + STEP);
         if (which < 2) {
             f32x2 xa[P], xb[P];
             Ln::unpack(u, v, xa, xb);
@@ -305,10 +316,10 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks) rotary_fwd_kernel(const 
             Ln::pack(xa, xb, u, v);
         }
         if (ln.on && h0 + slot < count) {
-            T* d = dst + h * r.dh;
-            *reinterpret_cast<uint4*>(d + ln.ea) = u;
-            *reinterpret_cast<uint4*>(d + ln.eb) = v;
+            *reinterpret_cast<uint4*>(dst) = u;
+            *reinterpret_cast<uint4*>(dst + apart) = v;
         }
+        dst += dst_step;
     }
 }
 
@@ -327,6 +338,8 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSM) rotary_bwd_kernel(const _
     const uint32_t warps = (which ? gridDim.x - q_blocks : q_blocks) * (kThreads / 32);
     const bool norm = r.w;
     const Ln ln(a, sub);
+    const int apart = ln.apart(), heads = r.H;
+    const int64_t x_head = r.sh, g_head = a.dyh[which], d_head = r.dh, gb_stride = a.dyb[which], gl_stride = a.dyl[which];
     f32x2 dwa[P], dwb[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) dwa[i] = dwb[i] = pk2(0.f, 0.f);
@@ -334,20 +347,22 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSM) rotary_bwd_kernel(const _
     __syncthreads();
     for (uint32_t t = (blockIdx.x - (which ? q_blocks : 0)) * (kThreads / 32) + warp; t < tokens; t += warps) {
         const uint32_t b = t / L, l = t - b * L;
-        const T* xp = static_cast<const T*>(r.src) + b * r.sb + l * r.sl;
-        const T* gp = static_cast<const T*>(a.dy[which]) + b * a.dyb[which] + l * a.dyl[which];
-        T* dp = static_cast<T*>(r.dst) + b * r.db + l * r.dl;
+        const T* const x0 = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + ln.ea;
+        const T* const g0 = static_cast<const T*>(a.dy[which]) + b * gb_stride + l * gl_stride + ln.ea;
+        const T *xp = x0 + slot * x_head, *gp = g0 + slot * g_head;
+        T* dp = static_cast<T*>(r.dst) + b * r.db + l * r.dl + slot * d_head + ln.ea;
         stage_turns<N, LANES>(a, s_turn[warp], load_pos(a, b, l));
-        for (int h0 = 0; h0 < r.H; h0 += STEP) {
-            // (a lane behind the last head reads that one again: every address lies inside the rows)
-            const bool mine = ln.on && h0 + slot < r.H;
-            const int h = h0 + slot < r.H ? h0 + slot : r.H - 1;
-            const T* g = gp + h * a.dyh[which];
-            uint4 ga = *reinterpret_cast<const uint4*>(g + ln.ea), gb = *reinterpret_cast<const uint4*>(g + ln.eb);
+        for (int h0 = 0; h0 < heads; h0 += STEP) {
+            // (a lane behind the last head reads the first: every address lies inside the rows)
+            const bool in = h0 + slot < heads, mine = ln.on && in;
+            const T* g = in ? gp : g0;
+            uint4 ga = *reinterpret_cast<const uint4*>(g), gb = *reinterpret_cast<const uint4*>(g + apart);
+            gp += STEP * g_head;
             f32x2 da[P], db[P];
             if (norm) {
-                const T* x = xp + h * r.sh;
-                const uint4 va = *reinterpret_cast<const uint4*>(x + ln.ea), vb = *reinterpret_cast<const uint4*>(x + ln.eb);
+                const T* x = in ? xp : x0;
+                const uint4 va = *reinterpret_cast<const uint4*>(x), vb = *reinterpret_cast<const uint4*>(x + apart);
+                xp += STEP * x_head;
                 f32x2 xa[P], xb[P];
                 Ln::unpack(va, vb, xa, xb);
                 const float ss = group_sum<LANES>(ln.on ? Ln::squares(xa, xb) : 0.f);
@@ -383,10 +398,10 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSM) rotary_bwd_kernel(const _
             }
             if (mine) {
                 Ln::pack(da, db, ga, gb);
-                T* d = dp + h * r.dh;
-                *reinterpret_cast<uint4*>(d + ln.ea) = ga;
-                *reinterpret_cast<uint4*>(d + ln.eb) = gb;
+                *reinterpret_cast<uint4*>(dp) = ga;
+                *reinterpret_cast<uint4*>(dp + apart) = gb;
             }
+            dp += STEP * d_head;
         }
     }
     // the sums of a lane's values: over the warp's rows, then the warps
@@ -591,9 +606,9 @@ int launch_fwd(const RotArgs& a, int64_t io, cudaStream_t s, const char* who) {
         VTX_DISPATCH_IO(io, T, rotary_fwd_any_kernel<T><<<(unsigned)blocks, kThreads, 0, s>>>(a));
         return check_launch(who);
     }
-    // up to eight steps a warp once that still gives every SM its warps; below, fewer, down to one
+    // up to four steps a warp once that still gives every SM its warps; below, fewer, down to one
     const int step = 32 / lanes;
-    int steps = 8;
+    int steps = 4;
     auto chunks = [&](int h) { return (int)ceil_div<int64_t>(h, steps * step); };
     auto per_token = [&] { return (int64_t)chunks(a.r[0].H) + chunks(a.r[1].H) + chunks(a.r[2].H); };
     while (steps > 1 && tokens * per_token() < (int64_t)kNumSMs * kFwdBlocks * (kThreads / 32)) steps /= 2;
