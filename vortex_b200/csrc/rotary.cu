@@ -53,7 +53,7 @@ struct RotArgs {
 
 constexpr int kThreads = 256;
 constexpr int kMaxD = 512;
-constexpr int kFwdBlocks = 5, kBwdPerSM = 3, kTokenCost = 1;
+constexpr int kFwdBlocks = 5, kBwdPerSM = 2, kTokenCost = 1;
 constexpr int kBwdBlocks = kNumSMs * 4;
 
 __device__ __forceinline__ int64_t load_pos(const RotArgs& a, int64_t b, int64_t l) {
@@ -339,30 +339,60 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSM) rotary_bwd_kernel(const _
     const bool norm = r.w;
     const Ln ln(a, sub);
     const int apart = ln.apart(), heads = r.H;
-    const int64_t x_head = r.sh, g_head = a.dyh[which], d_head = r.dh, gb_stride = a.dyb[which], gl_stride = a.dyl[which];
+    const int64_t x_head = r.sh, g_head = a.dyh[which], d_head = r.dh;
     f32x2 dwa[P], dwb[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) dwa[i] = dwb[i] = pk2(0.f, 0.f);
     stage_weights<T, INTER, LANES>(a, r, s_w);
     __syncthreads();
-    for (uint32_t t = (blockIdx.x - (which ? q_blocks : 0)) * (kThreads / 32) + warp; t < tokens; t += warps) {
+    const T *x0 = nullptr, *g0 = nullptr, *xp = nullptr, *gp = nullptr;     // a token's first head, and the lane's next
+    uint4 nga, ngb, nva, nvb;                                      // loaded a step ahead, across tokens
+    auto begin = [&](uint32_t t) {
         const uint32_t b = t / L, l = t - b * L;
-        const T* const x0 = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + ln.ea;
-        const T* const g0 = static_cast<const T*>(a.dy[which]) + b * gb_stride + l * gl_stride + ln.ea;
-        const T *xp = x0 + slot * x_head, *gp = g0 + slot * g_head;
+        x0 = static_cast<const T*>(r.src) + b * r.sb + l * r.sl + ln.ea;
+        g0 = static_cast<const T*>(a.dy[which]) + b * a.dyb[which] + l * a.dyl[which] + ln.ea;
+        xp = x0 + slot * x_head;
+        gp = g0 + slot * g_head;
+    };
+    // (a lane behind the last head reads the first: every address lies inside the rows)
+    auto fetch = [&](int h0) {
+        const bool in = h0 + STEP <= heads || h0 + slot < heads;
+        const T* g = in ? gp : g0;
+        nga = *reinterpret_cast<const uint4*>(g);
+        ngb = *reinterpret_cast<const uint4*>(g + apart);
+        gp += STEP * g_head;
+        if (norm) {
+            const T* x = in ? xp : x0;
+            nva = *reinterpret_cast<const uint4*>(x);
+            nvb = *reinterpret_cast<const uint4*>(x + apart);
+            xp += STEP * x_head;
+        }
+    };
+    const uint32_t t0 = (blockIdx.x - (which ? q_blocks : 0)) * (kThreads / 32) + warp;
+    int64_t next_pos = 0;
+    if (t0 < tokens) {
+        begin(t0);
+        fetch(0);
+        next_pos = load_pos(a, t0 / L, t0 % L);
+    }
+    for (uint32_t t = t0; t < tokens; t += warps) {
+        const uint32_t b = t / L, l = t - b * L, n = t + warps;
         T* dp = static_cast<T*>(r.dst) + b * r.db + l * r.dl + slot * d_head + ln.ea;
-        stage_turns<N, LANES>(a, s_turn[warp], load_pos(a, b, l));
+        const int64_t pos = next_pos;
+        if (n < tokens) next_pos = load_pos(a, n / L, n % L);
+        stage_turns<N, LANES>(a, s_turn[warp], pos);
         for (int h0 = 0; h0 < heads; h0 += STEP) {
-            // (a lane behind the last head reads the first: every address lies inside the rows)
-            const bool in = h0 + slot < heads, mine = ln.on && in;
-            const T* g = in ? gp : g0;
-            uint4 ga = *reinterpret_cast<const uint4*>(g), gb = *reinterpret_cast<const uint4*>(g + apart);
-            gp += STEP * g_head;
+            const bool mine = ln.on && h0 + slot < heads;
+            uint4 ga = nga, gb = ngb;
+            const uint4 va = nva, vb = nvb;
+            if (h0 + STEP < heads) {
+                fetch(h0 + STEP);
+            } else if (n < tokens) {
+                begin(n);
+                fetch(0);
+            }
             f32x2 da[P], db[P];
             if (norm) {
-                const T* x = in ? xp : x0;
-                const uint4 va = *reinterpret_cast<const uint4*>(x), vb = *reinterpret_cast<const uint4*>(x + apart);
-                xp += STEP * x_head;
                 f32x2 xa[P], xb[P];
                 Ln::unpack(va, vb, xa, xb);
                 const float ss = group_sum<LANES>(ln.on ? Ln::squares(xa, xb) : 0.f);
