@@ -5,7 +5,7 @@
 // in one pass over the cache with a running maximum m.  Every key and value is read once for up to 16 query heads, two
 // operations a byte and head: memory bounds it.  What the kernels are built around:
 //
-// * Work.  The cache is cut into units of 64 keys of one key head; the units of all sequences and heads, in a row, are dealt
+// * Work.  The cache is cut into units of 64 or 128 keys of one key head; the units of all sequences and heads, in a row, are dealt
 //   out to the blocks in equal runs, whatever the lengths (they are on the device: every block sums them up itself).  A run
 //   covers the end of one (sequence, head), some whole ones, and the beginning of another; whole ones are finished in place,
 //   the two open ones leave (m, sum, unnormalised out) in the scratch, which the second kernel joins.  At most two open ones a
@@ -30,12 +30,18 @@ VTX_DEFINE_STATUS_READER()
 namespace vtx {
 namespace {
 
-constexpr int kThreads = 128, kWarps = 4, kTile = 16, kUnit = kWarps * kTile;
+constexpr int kThreads = 128, kWarps = 4, kTile = 16;
+// Tiles of 16 keys that a warp has in flight together: two of the smaller heads are as many bytes as one of the larger.
+constexpr int tiles(int DP) { return DP == 64 ? 2 : 1; }
+// Keys of a unit of work, in the tensor-core kernel and in the other.
+constexpr int unit_keys(int DP, bool tensor) { return kWarps * kTile * (tensor ? tiles(DP) : 1); }
 // Reference m of a running sum: p = exp2(s - m).  The largest score seen stays between m + shift and m + shift + slack.
 // fp16 keeps nothing below 2^-25: its probabilities are held near the top of its range (at most 2^15), so that even 2^20 keys
 // of 2^-25 of the largest one's weight still count; bf16 and fp32 need no shift.
-template <typename T> struct Ref { static constexpr float shift = 0.f, slack = 8.f; };
-template <> struct Ref<__half> { static constexpr float shift = 11.f, slack = 4.f; };
+template <typename T> struct Ref {
+    static constexpr bool half = DTypeCode<T>::value == VTX_F16;
+    static constexpr float shift = half ? 11.f : 0.f, slack = half ? 4.f : 8.f;
+};
 
 struct AttnArgs {
     const void* q;
@@ -57,6 +63,7 @@ struct AttnArgs {
     int window;                     // INT_MAX: none
     int B, Hq, G, D, page_size, num_pages;
     int passes, head_groups;        // passes over the G query heads of a key head; Hk * passes
+    int unit;                       // keys of a unit of work
     int64_t max_keys;
 };
 
@@ -78,7 +85,7 @@ struct Seq {                        // keys lo .. n-1 of a sequence; tiles start
         lo = (len > a.window) ? len - a.window : 0;
         if (lo > n) lo = n;
         base = lo & ~(kTile - 1);
-        units = n > base ? (n - base + kUnit - 1) / kUnit : 1;      // an empty one has a unit, to write its zeros
+        units = n > base ? (n - base + a.unit - 1) / a.unit : 1;      // an empty one has a unit, to write its zeros
     }
 };
 
@@ -116,6 +123,17 @@ struct Run {
         __shared__ int64_t s_tot[kWarps], s_first;
         __shared__ int s_b;
         const int tid = threadIdx.x;
+        if (a.B <= 32) {                    // every warp for itself
+            const int lane = tid & 31;
+            const int64_t own = lane < a.B ? (int64_t)Seq(a, lane).units * a.head_groups : 0, incl = warp_scan(own);
+            units = __shfl_sync(0xffffffffu, incl, 31);
+            at = run_start(units, blockIdx.x, gridDim.x);
+            end = run_start(units, blockIdx.x + 1, gridDim.x);
+            const unsigned in = __ballot_sync(0xffffffffu, at >= incl - own && at < incl);
+            b = in ? __ffs(in) - 1 : 0;
+            seq_first = __shfl_sync(0xffffffffu, incl - own, b);
+            return;
+        }
         int64_t mine = tid < a.B ? (int64_t)Seq(a, tid).units * a.head_groups : 0, total, incl;
         incl = block_scan(mine, s_tot, total);
         units = total;
@@ -252,13 +270,14 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 
 // Where the 16 rows of a tile lie.  IN_PAGE (page size a multiple of 16, or no table): one page and slot.  Else: lane r holds
 // those of row r.  Looked up a batch of tiles at a time, and the batch after it already, so that no tile waits for the table.
-template <bool IN_PAGE> struct Pages {
-    static constexpr int kBatch = IN_PAGE ? 32 : 2;      // units per batch
+template <bool IN_PAGE, int KT> struct Pages {
+    static constexpr int kBatch = IN_PAGE ? 32 / KT : 2 / KT;      // units per batch
     int id, slot, next_id, next_slot;                    // of this lane's tile or row
     __device__ void fetch(const AttnArgs& a, const Piece& p, int c, int warp, int& page, int& at) const {
         const int lane = threadIdx.x & 31;
-        const int unit = c + (IN_PAGE ? lane : lane >> 4);
-        const int64_t pos = (int64_t)p.base + ((int64_t)unit * kWarps + warp) * kTile + (IN_PAGE ? 0 : lane & 15);
+        const int tile = IN_PAGE ? lane : lane >> 4;     // of the batch's, KT to a unit
+        const int unit = c + tile / KT;
+        const int64_t pos = (int64_t)p.base + (((int64_t)unit * kWarps + warp) * KT + tile % KT) * kTile + (IN_PAGE ? 0 : lane & 15);
         page = -1;
         at = 0;
         if (unit < p.c1 && pos < p.n && (IN_PAGE || pos >= p.lo)) {
@@ -277,18 +296,17 @@ template <bool IN_PAGE> struct Pages {
     }
 };
 
-template <typename T, int DP, int NT, bool IN_PAGE> struct Tile {
-    // rows: keys 0..15 of the tile; mask: which of them count
-    uint32_t mask;
+template <bool IN_PAGE> struct Tile {
+    uint32_t mask;                        // which of its 16 keys count
     int64_t ko, vo;                       // IN_PAGE: offset of row 0
     int64_t krow[2], vrow[4];             // else: offsets of the lane's rows
 };
 
-constexpr int decode_blocks_per_sm(int DP, int NT) { return DP == 64 ? (NT == 1 ? 5 : 4) : DP == 128 ? (NT == 1 ? 3 : 2) : 2; }
+constexpr int decode_blocks_per_sm(int DP, int NT) { return DP == 64 ? (NT == 1 ? 4 : 3) : DP == 128 ? (NT == 1 ? 3 : 2) : 2; }
 
 template <typename T, int DP, int NT, bool IN_PAGE>
 __global__ void __launch_bounds__(kThreads, decode_blocks_per_sm(DP, NT)) decode_kernel(const __grid_constant__ AttnArgs a) {
-    constexpr int HP = 8 * NT, KC = DP / 32, VC = DP / 64, MT = DP / 16, PITCH = DP + 4;
+    constexpr int HP = 8 * NT, KC = DP / 32, VC = DP / 64, MT = DP / 16, PITCH = DP + 4, KT = tiles(DP);
     __shared__ __align__(16) float s_o[kWarps * HP * PITCH];
     __shared__ float s_m[kWarps][HP], s_l[kWarps][HP];
     asm volatile("griddepcontrol.launch_dependents;");
@@ -320,163 +338,179 @@ __global__ void __launch_bounds__(kThreads, decode_blocks_per_sm(DP, NT)) decode
         }
         const T* kh = kp + p.kvh * a.ksh + t * 8;
         const T* vh = vp + p.kvh * a.vsh + g * 8;
-        uint4 kr[KC][2], vr[VC][4];
-        Pages<IN_PAGE> pages;
+        uint4 kr[KT][KC][2], vr[KT][VC][4];
+        Pages<IN_PAGE, KT> pages;
         pages.fetch(a, p, p.c0, warp, pages.id, pages.slot);
         pages.fetch(a, p, p.c0 + pages.kBatch, warp, pages.next_id, pages.next_slot);
         int left = pages.kBatch;
 
-        // rows of unit c's tile; moves the lookups on
-        auto locate = [&](int c) {
-            Tile<T, DP, NT, IN_PAGE> tl;
+        // the warp's tiles of unit c; moves the lookups on
+        auto locate = [&](int c, Tile<IN_PAGE> (&tl)[KT]) {
             if (left == 0) {
                 pages.id = pages.next_id; pages.slot = pages.next_slot;
                 pages.fetch(a, p, c + pages.kBatch, warp, pages.next_id, pages.next_slot);
                 left = pages.kBatch;
             }
-            const int j = pages.kBatch - left--;
-            const int64_t pos = (int64_t)p.base + ((int64_t)c * kWarps + warp) * kTile;
-            if (IN_PAGE) {
-                const int id = __shfl_sync(0xffffffffu, pages.id, j), slot = __shfl_sync(0xffffffffu, pages.slot, j);
-                tl.mask = 0;
-                if (id >= 0) {
-                    const int64_t from = p.lo - pos, to = p.n - pos;          // rows from .. to - 1
-                    tl.mask = to >= 16 ? 0xffffu : (1u << to) - 1u;            // (to > 0 where there is a page)
-                    if (from > 0) tl.mask &= from >= 16 ? 0u : 0xffffu << from;
-                }
-                tl.ko = (int64_t)id * a.ksp + (int64_t)slot * a.kss;
-                tl.vo = (int64_t)id * a.vsp + (int64_t)slot * a.vss;
-            } else {
-                const int at = j * 16;
-                tl.mask = (__ballot_sync(0xffffffffu, pages.id >= 0) >> at) & 0xffffu;
+            const int j = (pages.kBatch - left--) * KT;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = at + g + 8 * i;
-                    tl.krow[i] = (int64_t)__shfl_sync(0xffffffffu, pages.id, r) * a.ksp + (int64_t)__shfl_sync(0xffffffffu, pages.slot, r) * a.kss;
-                }
+            for (int x = 0; x < KT; ++x) {
+                if (IN_PAGE) {
+                    const int64_t pos = (int64_t)p.base + (((int64_t)c * kWarps + warp) * KT + x) * kTile;
+                    const int id = __shfl_sync(0xffffffffu, pages.id, j + x), slot = __shfl_sync(0xffffffffu, pages.slot, j + x);
+                    tl[x].mask = 0;
+                    if (id >= 0) {
+                        const int64_t from = p.lo - pos, to = p.n - pos;          // rows from .. to - 1
+                        tl[x].mask = to >= 16 ? 0xffffu : (1u << to) - 1u;         // (to > 0 where there is a page)
+                        if (from > 0) tl[x].mask &= from >= 16 ? 0u : 0xffffu << from;
+                    }
+                    tl[x].ko = (int64_t)id * a.ksp + (int64_t)slot * a.kss;
+                    tl[x].vo = (int64_t)id * a.vsp + (int64_t)slot * a.vss;
+                } else {
+                    const int at = (j + x) * 16;
+                    tl[x].mask = (__ballot_sync(0xffffffffu, pages.id >= 0) >> at) & 0xffffu;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = at + 2 * t + (i & 1) + 8 * (i >> 1);
-                    tl.vrow[i] = (int64_t)__shfl_sync(0xffffffffu, pages.id, r) * a.vsp + (int64_t)__shfl_sync(0xffffffffu, pages.slot, r) * a.vss;
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = at + g + 8 * i;
+                        tl[x].krow[i] = (int64_t)__shfl_sync(0xffffffffu, pages.id, r) * a.ksp + (int64_t)__shfl_sync(0xffffffffu, pages.slot, r) * a.kss;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = at + 2 * t + (i & 1) + 8 * (i >> 1);
+                        tl[x].vrow[i] = (int64_t)__shfl_sync(0xffffffffu, pages.id, r) * a.vsp + (int64_t)__shfl_sync(0xffffffffu, pages.slot, r) * a.vss;
+                    }
                 }
             }
-            return tl;
         };
         // Rows that do not count are not read, and enter as zeros: whatever lies there stays out.
-        auto load_k = [&](const Tile<T, DP, NT, IN_PAGE>& tl) {
+        auto load_k = [&](const Tile<IN_PAGE> (&tl)[KT]) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const T* row = kh + (IN_PAGE ? tl.ko + (g + 8 * r) * a.kss : tl.krow[r]);
-                if (tl.mask == 0xffffu && full_d) {
+            for (int x = 0; x < KT; ++x)
 #pragma unroll
-                    for (int i = 0; i < KC; ++i) kr[i][r] = ld16(row + i * 32);
-                } else {
-                    const bool ok = (tl.mask >> (g + 8 * r)) & 1;
+                for (int r = 0; r < 2; ++r) {
+                    const T* row = kh + (IN_PAGE ? tl[x].ko + (g + 8 * r) * a.kss : tl[x].krow[r]);
+                    if (tl[x].mask == 0xffffu && full_d) {
 #pragma unroll
-                    for (int i = 0; i < KC; ++i) {
-                        kr[i][r] = make_uint4(0, 0, 0, 0);
-                        if (ok && i * 32 + t * 8 < a.D) kr[i][r] = ld16(row + i * 32);
+                        for (int i = 0; i < KC; ++i) kr[x][i][r] = ld16(row + i * 32);
+                    } else {
+                        const bool ok = (tl[x].mask >> (g + 8 * r)) & 1;
+#pragma unroll
+                        for (int i = 0; i < KC; ++i) {
+                            kr[x][i][r] = make_uint4(0, 0, 0, 0);
+                            if (ok && i * 32 + t * 8 < a.D) kr[x][i][r] = ld16(row + i * 32);
+                        }
                     }
                 }
-            }
         };
-        auto load_v = [&](const Tile<T, DP, NT, IN_PAGE>& tl) {
+        auto load_v = [&](const Tile<IN_PAGE> (&tl)[KT]) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = 2 * t + (r & 1) + 8 * (r >> 1);
-                const T* row = vh + (IN_PAGE ? tl.vo + key * a.vss : tl.vrow[r]);
-                if (tl.mask == 0xffffu && full_d) {
+            for (int x = 0; x < KT; ++x)
 #pragma unroll
-                    for (int i = 0; i < VC; ++i) vr[i][r] = ld16(row + i * 64);
-                } else {
-                    const bool ok = (tl.mask >> key) & 1;
+                for (int r = 0; r < 4; ++r) {
+                    const int key = 2 * t + (r & 1) + 8 * (r >> 1);
+                    const T* row = vh + (IN_PAGE ? tl[x].vo + key * a.vss : tl[x].vrow[r]);
+                    if (tl[x].mask == 0xffffu && full_d) {
 #pragma unroll
-                    for (int i = 0; i < VC; ++i) {
-                        vr[i][r] = make_uint4(0, 0, 0, 0);
-                        if (ok && i * 64 + g * 8 < a.D) vr[i][r] = ld16(row + i * 64);
+                        for (int i = 0; i < VC; ++i) vr[x][i][r] = ld16(row + i * 64);
+                    } else {
+                        const bool ok = (tl[x].mask >> key) & 1;
+#pragma unroll
+                        for (int i = 0; i < VC; ++i) {
+                            vr[x][i][r] = make_uint4(0, 0, 0, 0);
+                            if (ok && i * 64 + g * 8 < a.D) vr[x][i][r] = ld16(row + i * 64);
+                        }
                     }
                 }
-            }
         };
 
-        Tile<T, DP, NT, IN_PAGE> cur = locate(p.c0);
+        Tile<IN_PAGE> cur[KT];
+        locate(p.c0, cur);
         load_k(cur);
         load_v(cur);
         for (int c = p.c0; c < p.c1; ++c) {
-            float s[NT][4];
+            float s[KT][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            for (int x = 0; x < KT; ++x)
 #pragma unroll
-                for (int i = 0; i < KC; ++i) {
-                    mma<T>(s[nt], kr[i][0].x, kr[i][1].x, kr[i][0].y, kr[i][1].y, qf[i][nt].x, qf[i][nt].y);
-                    mma<T>(s[nt], kr[i][0].z, kr[i][1].z, kr[i][0].w, kr[i][1].w, qf[i][nt].z, qf[i][nt].w);
+                for (int nt = 0; nt < NT; ++nt) {
+                    s[x][nt][0] = s[x][nt][1] = s[x][nt][2] = s[x][nt][3] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < KC; ++i) {
+                        mma<T>(s[x][nt], kr[x][i][0].x, kr[x][i][1].x, kr[x][i][0].y, kr[x][i][1].y, qf[i][nt].x, qf[i][nt].y);
+                        mma<T>(s[x][nt], kr[x][i][0].z, kr[x][i][1].z, kr[x][i][0].w, kr[x][i][1].w, qf[i][nt].z, qf[i][nt].w);
+                    }
                 }
-            }
-            Tile<T, DP, NT, IN_PAGE> nxt;
+            Tile<IN_PAGE> nxt[KT];
             const bool more = c + 1 < p.c1;
             if (more) {
-                nxt = locate(c + 1);
+                locate(c + 1, nxt);
                 load_k(nxt);
             }
             bool up = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int x = 0; x < KT; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] *= a.scale;
-                if (cur.mask != 0xffffu) {
-                    if (!((cur.mask >> g) & 1)) s[nt][0] = s[nt][1] = -INFINITY;
-                    if (!((cur.mask >> (g + 8)) & 1)) s[nt][2] = s[nt][3] = -INFINITY;
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[x][nt][i] *= a.scale;
+                    if (cur[x].mask != 0xffffu) {
+                        if (!((cur[x].mask >> g) & 1)) s[x][nt][0] = s[x][nt][1] = -INFINITY;
+                        if (!((cur[x].mask >> (g + 8)) & 1)) s[x][nt][2] = s[x][nt][3] = -INFINITY;
+                    }
+                    constexpr float over = Ref<T>::shift + Ref<T>::slack;
+                    up |= fmaxf(s[x][nt][0], s[x][nt][2]) > m[nt][0] + over || fmaxf(s[x][nt][1], s[x][nt][3]) > m[nt][1] + over;
                 }
-                constexpr float over = Ref<T>::shift + Ref<T>::slack;
-                up |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + over || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + over;
-            }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float x = fmaxf(s[nt][i], s[nt][i + 2]);
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        x = fmaxf(x - Ref<T>::shift, m[nt][i]);
-                        const float f = exp2f(m[nt][i] - x);
-                        m[nt][i] = x;
+                        float z = fmaxf(s[0][nt][i], s[0][nt][i + 2]);
+#pragma unroll
+                        for (int x = 1; x < KT; ++x) z = fmaxf(z, fmaxf(s[x][nt][i], s[x][nt][i + 2]));
+                        z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 4));
+                        z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 8));
+                        z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 16));
+                        z = fmaxf(z - Ref<T>::shift, m[nt][i]);
+                        const float f = exp2f(m[nt][i] - z);
+                        m[nt][i] = z;
                         l[nt][i] *= f;
 #pragma unroll
                         for (int j = 0; j < MT; ++j) { o[j][nt][i] *= f; o[j][nt][i + 2] *= f; }
                     }
             }
-            uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int x = 0; x < KT; ++x) {
+                uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float p0 = exp2f(s[nt][2 * i] - m[nt][0]), p1 = exp2f(s[nt][2 * i + 1] - m[nt][1]);
-                    l[nt][0] += p0;
-                    l[nt][1] += p1;
-                    const uint32_t hi = pack2<T>(p0, p1);
-                    const float2 back = unpack2<T>(hi);
-                    ph[nt][i] = transpose8(hi);
-                    pl[nt][i] = transpose8(pack2<T>(p0 - back.x, p1 - back.y));
-                }
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < VC; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t r0 = word(vr[i][0], j), r1 = word(vr[i][1], j), r2 = word(vr[i][2], j), r3 = word(vr[i][3], j);
-                    const uint32_t a0 = __byte_perm(r0, r1, 0x5410), a1 = __byte_perm(r0, r1, 0x7632);
-                    const uint32_t a2 = __byte_perm(r2, r3, 0x5410), a3 = __byte_perm(r2, r3, 0x7632);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma<T>(o[i * 4 + j][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-                        mma<T>(o[i * 4 + j][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                    for (int i = 0; i < 2; ++i) {
+                        const float p0 = exp2f(s[x][nt][2 * i] - m[nt][0]), p1 = exp2f(s[x][nt][2 * i + 1] - m[nt][1]);
+                        l[nt][0] += p0;
+                        l[nt][1] += p1;
+                        const uint32_t hi = pack2<T>(p0, p1);
+                        const float2 back = unpack2<T>(hi);
+                        ph[nt][i] = transpose8(hi);
+                        pl[nt][i] = transpose8(pack2<T>(p0 - back.x, p1 - back.y));
                     }
-                }
+#pragma unroll
+                for (int i = 0; i < VC; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t r0 = word(vr[x][i][0], j), r1 = word(vr[x][i][1], j), r2 = word(vr[x][i][2], j), r3 = word(vr[x][i][3], j);
+                        const uint32_t a0 = __byte_perm(r0, r1, 0x5410), a1 = __byte_perm(r0, r1, 0x7632);
+                        const uint32_t a2 = __byte_perm(r2, r3, 0x5410), a3 = __byte_perm(r2, r3, 0x7632);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma<T>(o[i * 4 + j][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+                            mma<T>(o[i * 4 + j][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+                        }
+                    }
+            }
             if (more) {
                 load_v(nxt);
-                cur = nxt;
+#pragma unroll
+                for (int x = 0; x < KT; ++x) cur[x] = nxt[x];
             }
         }
 
@@ -595,7 +629,7 @@ __global__ void __launch_bounds__(kThreads) decode_any_kernel(const __grid_const
                         s += __shfl_xor_sync(0xffffffffu, s, 2);
                         s += __shfl_xor_sync(0xffffffffu, s, 4);
                         s = ok[u] ? s * a.scale : -INFINITY;
-                        if (s > m[h] + Ref<float>::slack) {
+                        if (s > m[h] + Ref<float>::shift + Ref<float>::slack) {
                             const float f = exp2f(m[h] - s);
                             m[h] = s;
                             l[h] *= f;
@@ -639,11 +673,10 @@ __global__ void __launch_bounds__(kThreads) decode_any_kernel(const __grid_const
 // ---- the open (sequence, head group)s: block (w, h) joins head h of the one that begins in run w ----------------------------
 template <typename T, int DP, int HP> __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ AttnArgs a, int W) {
     constexpr int Q = DP / 4, R = kThreads / Q;                      // threads to a row of sums; rows at a time
-    extern __shared__ float s_f[];                                   // [W] factors
-    __shared__ float s_red[2][kWarps];
+    __shared__ float2 s_ml[R];
     __shared__ __align__(16) float s_o[R][DP];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int w0 = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int w0 = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
     const Open op = a.open[w0];
     if (op.b < 0) return;
     const int kvh = op.hg / a.passes, first = (op.hg - kvh * a.passes) * HP;
@@ -651,44 +684,33 @@ template <typename T, int DP, int HP> __global__ void __launch_bounds__(kThreads
     const int n = op.last - w0 + 1;
     // the run it begins in keeps it in slot 1, the others in slot 0; a run may be empty
     auto row = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i == 0)) * HP + h; };
+    const bool sparse = op.units < W;
     auto empty = [&](int i) { return run_start(op.units, w0 + i, W) == run_start(op.units, w0 + i + 1, W); };
-    float m = -FLT_MAX;
-    for (int i = tid; i < n; i += kThreads)
-        if (!empty(i)) m = fmaxf(m, a.part_ml[row(i)].x);
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) s_red[0][warp] = m;
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_red[0][w]);
-    float l = 0.f;
-    for (int i = tid; i < n; i += kThreads) {
-        float f = 0.f;
-        if (!empty(i)) {
-            const float2 ml = a.part_ml[row(i)];
-            f = exp2f(ml.x - m);
-            l += f * ml.y;
-        }
-        s_f[i] = f;
-    }
-    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) s_red[1][warp] = l;
-    __syncthreads();
-    l = 0.f;
-    for (int w = 0; w < kWarps; ++w) l += s_red[1][w];
     const int q = tid % Q, r0 = tid / Q;
+    float m = -FLT_MAX, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int i = r0; i < n; i += R) {
-        if (empty(i)) continue;
-        const float f = s_f[i];
+        if (sparse && empty(i)) continue;
+        const float2 ml = a.part_ml[row(i)];
         const float4 x = *reinterpret_cast<const float4*>(a.part + row(i) * DP + q * 4);
-        o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+        const float top = fmaxf(m, ml.x), f = exp2f(m - top), g = exp2f(ml.x - top);
+        o.x = o.x * f + x.x * g; o.y = o.y * f + x.y * g; o.z = o.z * f + x.z * g; o.w = o.w * f + x.w * g;
+        l = l * f + ml.y * g;
+        m = top;
     }
+    if (q == 0) s_ml[r0] = make_float2(m, l);
     *reinterpret_cast<float4*>(&s_o[r0][q * 4]) = o;
     __syncthreads();
+    m = -FLT_MAX;
+    for (int i = 0; i < R; ++i) m = fmaxf(m, s_ml[i].x);
+    l = 0.f;
+    for (int i = 0; i < R; ++i) l += s_ml[i].y * exp2f(s_ml[i].x - m);
     const int head = kvh * a.G + first + h;
     T* y = static_cast<T*>(a.out) + op.b * a.osb + head * a.osh;
     for (int d = tid; d < a.D; d += kThreads) {
         float x = 0.f;
-        for (int i = 0; i < R; ++i) x += s_o[i][d];
+        for (int i = 0; i < R; ++i) x += s_o[i][d] * exp2f(s_ml[i].x - m);
         y[d] = from_f32<T>(x / l);
     }
     if (tid == 0 && a.lse) a.lse[(int64_t)op.b * a.Hq + head] = (m + log2f(l)) * 0.69314718055994531f;
@@ -696,7 +718,7 @@ template <typename T, int DP, int HP> __global__ void __launch_bounds__(kThreads
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
 struct Plan {
-    int DP, HP, blocks;
+    int DP, HP, blocks, unit;
     bool tensor, in_page, vec;
     int64_t slots, bytes;
 };
@@ -728,7 +750,8 @@ Plan make_plan(const vtx_paged_decode_params& p) {
     }
     // no more blocks than units
     const int64_t keys = p.block_table ? p.table_width * p.page_size : p.page_size;
-    const int64_t per_seq = ceil_div<int64_t>(keys < INT32_MAX ? keys : INT32_MAX, kUnit) + 1;
+    pl.unit = unit_keys(pl.DP, pl.tensor);
+    const int64_t per_seq = ceil_div<int64_t>(keys < INT32_MAX ? keys : INT32_MAX, pl.unit) + 1;
     const int64_t pairs = p.B * p.Hk * ceil_div<int64_t>(G, pl.HP);
     int64_t most = pairs > (1 << 20) ? pairs : pairs * (per_seq > 0 ? per_seq : 1);
     pl.blocks = (int)(most < (int64_t)kNumSMs * per_sm ? most : (int64_t)kNumSMs * per_sm);
@@ -741,7 +764,6 @@ template <typename T, int DP, int HP> int launch_join(const AttnArgs& a, int W, 
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)W, (unsigned)(a.G < HP ? a.G : HP));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)W * sizeof(float);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -827,6 +849,7 @@ extern "C" int vtx_paged_decode_attention(const vtx_paged_decode_params* p, void
     a.B = (int)p->B; a.Hq = (int)p->Hq; a.G = (int)(p->Hq / p->Hk); a.D = (int)p->D;
     a.page_size = (int)p->page_size; a.num_pages = (int)p->num_pages;
     a.passes = (a.G + pl.HP - 1) / pl.HP;
+    a.unit = pl.unit;
     a.head_groups = (int)p->Hk * a.passes;
     a.max_keys = p->block_table ? p->table_width * p->page_size : p->page_size;
     cudaStream_t s = (cudaStream_t)stream;
