@@ -144,3 +144,113 @@ def test_frequencies():
             attn_ops.rotary_inv_freq(**kw)
     with pytest.raises(NotImplementedError):
         attn_ops.rotary_inv_freq(8, scaling="other")
+
+
+# ------------------------------------------------------------------ the cache's bookkeeping
+@pytest.fixture
+def host_copies(monkeypatch):
+    """The pages copied as the kernel copies them, all at the same time, in tensors of the host."""
+    from vortex_b200 import attn_ops
+
+    def copy_pages(pools, src, dst):
+        assert len(set(dst)) == len(dst) and not set(dst) & set(src)
+        for p in pools:
+            p[dst] = p[src]
+
+    monkeypatch.setattr(attn_ops, "copy_pages", copy_pages)
+
+
+def cache(**kw):
+    from vortex_b200 import PagedKVCache
+    base = dict(layers=2, num_pages=20, page_size=4, num_heads=1, head_dim=1, max_sequences=5, max_length=30, device="cpu", dtype=torch.float64)
+    return PagedKVCache(**{**base, **kw})
+
+
+def store(c, positions, rows, values):
+    for p, r, x in zip(positions.tolist(), rows.tolist(), values):
+        if p >= 0:
+            at = c.block_table[r, p // c.page_size]
+            for i, pool in enumerate(c.k + c.v):
+                pool[at, p % c.page_size] = x + i
+
+
+def held(c, row):
+    n = c.length(row)
+    at = torch.arange(n)
+    return [pool[c.block_table[row].long()[at // c.page_size], at % c.page_size].flatten().tolist() for pool in c.k + c.v]
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_cache_holds_what_its_sequences_stored(host_copies, seed):
+    """Random openings, growth, steps, forks, ends and compactions against lists of what each sequence stored."""
+    import random
+    rng = random.Random(seed)
+    c, model, fresh = cache(page_size=rng.choice([1, 3, 4, 8])), {}, 0
+    for _ in range(400):
+        what = rng.choice(["open", "extend", "extend", "step", "step", "fork", "free", "compact"])
+        rows = sorted(model)
+        try:
+            if what == "open":
+                model[c.open()] = []
+            elif what == "extend" and rows:
+                some = rng.sample(rows, rng.randint(1, len(rows)))
+                counts = [rng.randint(0, 6) for _ in some]
+                pos, seq = c.extend(some, counts)
+                vals = [1000.0 * (fresh + i) for i in range(sum(counts))]
+                fresh += len(vals)
+                store(c, pos, seq, vals)
+                at = 0
+                for r, n in zip(some, counts):
+                    model[r] += vals[at:at + n]
+                    at += n
+            elif what == "step":
+                some = None if rng.random() < 0.5 else rng.sample(rows, rng.randint(0, len(rows)))
+                c.step(some)
+                some = rows if some is None else some
+                vals = [1000.0 * (fresh + i) for i in range(5)]
+                fresh += 5
+                store(c, c.positions, torch.arange(5), vals)
+                for r in range(5):
+                    if r in some:
+                        model[r].append(vals[r])
+                    assert c.lengths[r] == (len(model[r]) if r in some else 0)
+                    assert c.positions[r] == (len(model[r]) - 1 if r in some else -1)
+            elif what == "fork" and rows:
+                r = rng.choice(rows)
+                model[c.fork(r)] = list(model[r])
+            elif what == "free" and rows:
+                r = rng.choice(rows)
+                c.free(r)
+                del model[r]
+            elif what == "compact":
+                n = c.compact()
+                assert n == 20 - c.unused_pages == len({p for r in model for p in c.pages(r)})
+                assert all(p < n for r in model for p in c.pages(r))
+        except (RuntimeError, ValueError) as e:
+            assert "needed, " in str(e) or "rows hold" in str(e) or "tokens of at most" in str(e), e
+        for r, vals in model.items():
+            assert c.length(r) == len(vals) and held(c, r) == [[x + i for x in vals] for i in range(4)]
+            assert c.block_table[r, len(c.pages(r)):].eq(-1).all()
+        assert c.unused_pages + len({p for r in model for p in c.pages(r)}) == 20
+    for r in list(model):
+        c.free(r)
+    assert c.unused_pages == 20 and c.block_table.eq(-1).all()
+
+
+def test_cache_refusals_change_nothing(host_copies):
+    c = cache(num_pages=3, max_sequences=2, max_length=9)
+    a = c.open()
+    c.extend([a], [6])
+    before = (c.pages(a), c.length(a), c.unused_pages, c.block_table.clone())
+    b = c.open()
+    for f, exc in ((lambda: c.open(), RuntimeError), (lambda: c.extend([a], [4]), ValueError), (lambda: c.extend([a, a], [1, 1]), ValueError),
+                   (lambda: c.extend([a, b], [1, 5]), RuntimeError), (lambda: c.extend([a], [-1]), ValueError), (lambda: c.extend([a], [1, 1]), ValueError),
+                   (lambda: c.step([7]), ValueError), (lambda: c.fork(a), RuntimeError), (lambda: c.free(5), ValueError)):
+        with pytest.raises(exc):
+            f()
+        assert (c.pages(a), c.length(a), c.unused_pages) == before[:3] and torch.equal(c.block_table, before[3]) and c.length(b) == 0
+    c.free(b)
+    with pytest.raises(ValueError, match="holds no sequence"):
+        c.free(b)
+    with pytest.raises(ValueError):
+        cache(page_size=0)

@@ -618,3 +618,122 @@ def test_refusals(A):
     q = x.clone().requires_grad_()
     g1 = torch.autograd.grad(R_(q, None, pos, fr, w).sum(), q, create_graph=True)[0]
     refused(RuntimeError, "does not require grad", lambda: torch.autograd.grad(g1.sum(), q))
+
+
+# ------------------------------------------------------------------ a run of them together
+@pytest.mark.parametrize("io,page", [("bf16", 16), ("f16", 5), ("f32", 16)])
+@pytest.mark.parametrize("rotated,window", [(True, 0), (True, 20), (False, 0)])
+def test_attention_layers_of_a_stack(A, io, page, rotated, window):
+    """Two layers: ragged prompts, captured decode steps, a fork, a sequence that ends, a compaction and more steps; every
+    output against softmax(q k) v in float64 over the keys and values as the layer stored them, which are checked apart."""
+    from vortex_b200 import AttentionInferenceEngine, PagedKVCache
+
+    g, dt, Hq, H, D, S = gen(21), DT[io], 6, 2, 64, 4
+    mk = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dt)  # noqa: E731
+    cache = PagedKVCache(2, 60, page, H, D, max_sequences=S, max_length=100, dtype=dt)
+    fr, scale = A.rotary_inv_freq(32, 1e4, scaling="yarn", factor=4.0, trained_length=64)
+    wq, wk = 1 + 0.2 * torch.randn(D, generator=g, device="cuda"), 1 + 0.2 * torch.randn(D, generator=g, device="cuda")
+    layers = [AttentionInferenceEngine(cache, i, fr if rotated else None, q_weight=wq if i else None, k_weight=wk if i else None, scale=scale,
+                                       interleaved=bool(i), window=window) for i in range(2)]
+    f64 = fr.cuda() if rotated else torch.zeros(0, dtype=torch.float64, device="cuda")
+    seen = [{}, {}]                      # [layer][row] -> k (turned, float64, as stored) and v
+
+    def turned(i, x, w, pos):
+        y, mag = R.norm_rotate(x.double(), w if i else None, pos, f64, bool(i), scale, EPS)
+        return y, R.norm_rotate_bound(y, mag, dt)
+
+    def stored(i, row):
+        n = cache.length(row)
+        return R.gather(cache.k[i], cache.block_table[row], n), R.gather(cache.v[i], cache.block_table[row], n)
+
+    def remember(i, row, k, pos, v):
+        kk, vv = stored(i, row)
+        y, b = turned(i, k, wk, pos)
+        lo = cache.length(row) - k.shape[0]
+        within(kk[lo:], y, b, "stored k")
+        assert torch.equal(vv[lo:], v)
+        if lo:
+            assert torch.equal(kk[:lo], seen[i][row][0]) and torch.equal(vv[:lo], seen[i][row][1])
+        seen[i][row] = (kk.clone(), vv.clone())
+
+    rows, counts = [cache.open() for _ in range(3)], [33, 1, 16]
+    pos, seq = cache.extend(rows, counts)
+    for i, layer in enumerate(layers):
+        q, k, v = mk(50, Hq, D), mk(50, H, D), mk(50, H, D)
+        qo, ko = layer.prefill(q, k, v, pos, seq)
+        y, b = turned(i, q, wq, pos)
+        within(qo, y, b, "prompt q")
+        at = 0
+        for r, n in zip(rows, counts):
+            assert torch.equal(ko[at:at + n], stored(i, r)[0])
+            remember(i, r, k[at:at + n], pos[at:at + n], v[at:at + n])
+            at += n
+
+    q, k, v = ([torch.zeros(S, h, D, device="cuda", dtype=dt) for _ in range(2)] for h in (Hq, H, H))
+    run = lambda: [layer.decode(q[i], k[i], v[i]) for i, layer in enumerate(layers)]  # noqa: E731
+    cache.step([])
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+
+    def step(some=None):
+        live = sorted(seen[0]) if some is None else some
+        cache.step(some)
+        for t in q + k + v:
+            t.copy_(mk(*t.shape))
+        graph.replay()
+        lens = [cache.length(r) if r in live else 0 for r in range(S)]
+        at = torch.tensor([max(n - 1, 0) for n in lens], device="cuda")
+        for i in range(2):
+            for r in live:
+                remember(i, r, k[i][r:r + 1], at[r:r + 1], v[i][r:r + 1])
+            y, b = turned(i, q[i], wq, at)
+            ref, _, bound = R.attend(y, cache.k[i], cache.v[i], cache.block_table, lens, D ** -0.5, window)
+            # the queries enter rounded: a change of q by b moves each score by at most sum b |k|, a probability by twice that
+            for r in live:
+                kk, vv = seen[i][r]
+                lo = max(0, lens[r] - window) if window else 0
+                kk, vv = kk[lo:].double().repeat_interleave(Hq // H, 1), vv[lo:].double().repeat_interleave(Hq // H, 1)
+                d = torch.einsum("hd,nhd->hn", b[r], kk.abs()).amax(-1) * D ** -0.5
+                bound[r] += 2 * torch.expm1(2 * d)[:, None] * vv.abs().amax(0)
+            within(outs[i], ref, bound + R.rounding(ref.abs() + bound, dt), f"layer {i}")
+
+    for _ in range(3):
+        step()
+    child = cache.fork(rows[0])
+    for i in range(2):
+        seen[i][child] = seen[i][rows[0]]
+    step()
+    step([rows[1], child])
+    cache.free(rows[1])
+    for i in range(2):
+        del seen[i][rows[1]]
+    assert cache.compact() == 60 - cache.unused_pages
+    for i in range(2):
+        for r in seen[i]:
+            assert all(torch.equal(a, b) for a, b in zip(stored(i, r), seen[i][r]))
+    for _ in range(2):
+        step()
+
+
+def test_cache_copies_on_the_current_stream(A):
+    """fork and compact are work of the current stream: what was stored before them is in the copies."""
+    from vortex_b200 import PagedKVCache
+    s = torch.cuda.Stream()
+    cache = PagedKVCache(1, 8, 4, 1, 8, max_sequences=3, max_length=16, dtype=torch.float32)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        a = cache.open()
+        b = cache.open()
+        pos, seq = cache.extend([a, b], [6, 2])
+        x = torch.randn(8, 1, 8, generator=gen(22), device="cuda")
+        torch.cuda._sleep(20_000_000)
+        A.rotary_append(x, x, x, pos, cache.k[0], cache.v[0], cache.block_table, seq_ids=seq)
+        c = cache.fork(a)
+        cache.free(a)
+        cache.compact()
+        got = [R.gather(cache.k[0], cache.block_table[r], cache.length(r)) for r in (b, c)]
+    s.synchronize()
+    assert torch.equal(got[0], x[6:]) and torch.equal(got[1], x[:6])

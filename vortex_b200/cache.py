@@ -9,15 +9,18 @@ dictionaries, keyed by layer index:
 Prefill writes the FIR caches in the activation dtype; every decode step returns them in fp32
 (``vortex/model/engine.py:427-449``).
 """
+import heapq
 from dataclasses import dataclass, field
-from typing import Optional
+from typing import Optional, Sequence
 
+import torch
 from torch import Tensor
 
 
 @dataclass
 class InferenceParams:
-    """Attention KV-cache bookkeeping (kept for interface parity; not touched by the Hyena engine)."""
+    """Attention KV-cache bookkeeping (kept for interface parity; not touched by the Hyena engine).  ``PagedKVCache`` below
+    is what ``AttentionInferenceEngine`` keeps its keys and values in."""
 
     max_seqlen: int
     max_batch_size: int
@@ -59,3 +62,187 @@ class HyenaCascadeFIRInferenceParams:
 
     def reset(self):
         self.fir_filter_length, self.fir_inner_filter_length, self.seqlen_offset = 3, 4, 0
+
+
+class PagedKVCache:
+    """Keys and values of a stack's attention layers, in pages of ``page_size`` tokens that the sequences share.
+
+    ``k[layer]``, ``v[layer]``: pools [num_pages, page_size, num_heads, head_dim].  A page number means the same page in
+    every pool: a sequence holds ``ceil(length / page_size)`` of them, listed in its row of ``block_table`` (int32
+    [max_sequences, max_length / page_size], -1 behind the last).  The numbers are kept on the host, where the planning is
+    done; the device holds the table, and for the step at work ``positions`` (int32 [max_sequences], the new token's, -1
+    where a row has none) and ``lengths`` (its keys, the new one included, 0 where a row has none).  These tensors keep their
+    addresses: a captured decode step follows what ``step`` puts there before each replay.
+
+    ``open`` / ``extend`` / ``step`` / ``free`` change the bookkeeping on the host and upload what changed on the current
+    stream; ``fork`` and ``compact`` copy pages as well (``attn_ops.copy_pages``).  None of them may run under stream
+    capture.  A call that raises has changed nothing.  Not thread-safe."""
+
+    def __init__(self, layers, num_pages, page_size, num_heads, head_dim, *, max_sequences, max_length, device="cuda",
+                 dtype=torch.bfloat16):
+        if min(layers, num_pages, page_size, num_heads, head_dim, max_sequences, max_length) < 1:
+            raise ValueError("a paged cache needs at least one of everything")
+        shape = (num_pages, page_size, num_heads, head_dim)
+        self.k = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
+        self.v = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(layers)]
+        self.page_size, self.num_pages, self.max_length = page_size, num_pages, max_length
+        width = -(-max_length // page_size)
+        self.block_table = torch.full((max_sequences, width), -1, device=device, dtype=torch.int32)
+        self._step = torch.zeros(2, max_sequences, device=device, dtype=torch.int32)
+        self._step[0] = -1
+        self.positions, self.lengths = self._step[0], self._step[1]
+        self._table = torch.full((max_sequences, width), -1, dtype=torch.int32)      # the host's copy
+        self._pages: list[Optional[list[int]]] = [None] * max_sequences              # of each open row
+        self._length = [0] * max_sequences
+        self._users = [0] * num_pages                                                # rows that hold a page
+        self._unused = list(range(num_pages))                                        # a heap: lowest numbers first
+
+    # -- what is there
+    def length(self, row: int) -> int:
+        self._check(row)
+        return self._length[row]
+
+    def pages(self, row: int) -> list[int]:
+        self._check(row)
+        return list(self._pages[row])
+
+    @property
+    def unused_pages(self) -> int:
+        return len(self._unused)
+
+    def _check(self, row):
+        if not 0 <= row < len(self._pages) or self._pages[row] is None:
+            raise ValueError(f"row {row} holds no sequence")
+
+    def _take(self) -> int:
+        page = heapq.heappop(self._unused)
+        self._users[page] = 1
+        return page
+
+    def _upload(self, rows: Sequence[int]) -> None:
+        """The rows' part of the table, in one copy.  (From pageable memory, which CUDA has read when the call returns: the
+        host's copy may change afterwards, and nothing waits for the stream.)"""
+        if rows:
+            lo, hi = min(rows), max(rows) + 1
+            self.block_table[lo:hi].copy_(self._table[lo:hi], non_blocking=True)
+
+    # -- sequences
+    def open(self) -> int:
+        """An empty sequence; returns its row."""
+        for row, pages in enumerate(self._pages):
+            if pages is None:
+                self._pages[row], self._length[row] = [], 0
+                return row
+        raise RuntimeError(f"all {len(self._pages)} rows hold sequences")
+
+    def _grow(self, rows, counts) -> None:
+        """Room for counts[i] more tokens of rows[i]: bookkeeping and table."""
+        if len(set(rows)) != len(rows):
+            raise ValueError("a row occurs twice")
+        need = 0
+        for row, n in zip(rows, counts):
+            self._check(row)
+            if n < 0 or self._length[row] + n > self.max_length:
+                raise ValueError(f"row {row}: {self._length[row]} + {n} tokens of at most {self.max_length}")
+            need += -(-(self._length[row] + n) // self.page_size) - len(self._pages[row])
+        if need > len(self._unused):
+            raise RuntimeError(f"{need} pages needed, {len(self._unused)} unused")
+        changed = []
+        for row, n in zip(rows, counts):
+            self._length[row] += n
+            pages = self._pages[row]
+            while len(pages) * self.page_size < self._length[row]:
+                self._table[row, len(pages)] = page = self._take()
+                pages.append(page)
+                if not changed or changed[-1] != row:
+                    changed.append(row)
+        self._upload(changed)
+
+    def extend(self, rows: Sequence[int], counts: Sequence[int]):
+        """Room for ``counts[i]`` new tokens of sequence ``rows[i]``; returns their positions and rows (int32, on the device),
+        all of the first sequence's, then the second's: what ``attn_ops.rotary_append`` takes for a (ragged) prompt."""
+        rows, counts = list(rows), list(counts)
+        if len(rows) != len(counts):
+            raise ValueError("one count for every row")
+        first = [self.length(row) for row in rows]
+        self._grow(rows, counts)
+        both = torch.empty(2, sum(counts), dtype=torch.int32)
+        at = 0
+        for row, start, n in zip(rows, first, counts):
+            both[0, at:at + n] = torch.arange(start, start + n, dtype=torch.int32)
+            both[1, at:at + n] = row
+            at += n
+        both = both.to(self.block_table.device, non_blocking=True)
+        return both[0], both[1]
+
+    def step(self, rows: Optional[Sequence[int]] = None) -> None:
+        """Room for one new token of each of ``rows`` (None: every open sequence); ``positions`` and ``lengths`` say so to
+        the decode step that follows."""
+        rows = [r for r, p in enumerate(self._pages) if p is not None] if rows is None else list(rows)
+        self._grow(rows, [1] * len(rows))
+        both = torch.zeros(2, len(self._pages), dtype=torch.int32)
+        both[0] = -1
+        for row in rows:
+            both[0, row], both[1, row] = self._length[row] - 1, self._length[row]
+        self._step.copy_(both, non_blocking=True)
+
+    def fork(self, row: int) -> int:
+        """A sequence that begins as a copy of ``row``: full pages are shared, an open last page is copied in every pool.
+        Returns its row."""
+        self._check(row)
+        open_page = self._length[row] % self.page_size != 0
+        if open_page and not self._unused:
+            raise RuntimeError("1 page needed, 0 unused")
+        child = self.open()
+        pages = list(self._pages[row])
+        if open_page:
+            from . import attn_ops
+
+            page = self._unused[0]
+            try:
+                attn_ops.copy_pages(self.k + self.v, [pages[-1]], [page])
+            except Exception:
+                self._pages[child] = None
+                raise
+            pages[-1] = self._take()
+        for page in pages[:-1] if open_page else pages:
+            self._users[page] += 1
+        self._pages[child], self._length[child] = pages, self._length[row]
+        self._table[child, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+        self._upload([child])
+        return child
+
+    def free(self, row: int) -> None:
+        """Ends a sequence; pages that no other sequence holds are unused again."""
+        self._check(row)
+        for page in self._pages[row]:
+            self._users[page] -= 1
+            if self._users[page] == 0:
+                heapq.heappush(self._unused, page)
+        self._pages[row], self._length[row] = None, 0
+        self._table[row] = -1
+        self._upload([row])
+
+    def compact(self) -> int:
+        """Moves the pages in use to the lowest numbers and returns how many there are: what lies behind them in the pools
+        is free to be given back or reused."""
+        from . import attn_ops
+
+        used = self.num_pages - len(self._unused)
+        src = [p for p in range(used, self.num_pages) if self._users[p]]
+        dst = sorted(p for p in self._unused if p < used)
+        if not src:
+            return used
+        attn_ops.copy_pages(self.k + self.v, src, dst)
+        to = dict(zip(src, dst))
+        changed = []
+        for row, pages in enumerate(self._pages):
+            if pages and any(p in to for p in pages):
+                self._pages[row] = pages = [to.get(p, p) for p in pages]
+                self._table[row, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+                changed.append(row)
+        for a, b in to.items():
+            self._users[b], self._users[a] = self._users[a], 0
+        self._unused = list(range(used, self.num_pages))
+        self._upload(changed)
+        return used

@@ -8,6 +8,9 @@ through the C ABI; tensors that are not on a CUDA device are rejected.
 On top of the drop-in surface the engine offers the fused entry points the reference's model
 code looks for but never defines (``vortex/model/layers.py:18-21``): see ``fused_prefill`` /
 ``fused_decode`` here and ``vortex_b200.hyena_ops``.
+
+``AttentionInferenceEngine`` is the same for the attention layers between the Hyena layers: positions, the paged
+cache and the decode step (``vortex_b200.attn_ops``, ``vortex_b200.cache.PagedKVCache``).
 """
 from __future__ import annotations
 
@@ -261,3 +264,45 @@ class HyenaInferenceEngine:
             inference_params.state_dict[i] = st
         inference_params.fir_state_dict[i] = fs
         return y
+
+
+class AttentionInferenceEngine:
+    """One attention layer of a striped stack on a ``PagedKVCache``: what the reference's ``MHA`` does between its
+    projections (``vortex/model/attention.py:352-381,582``), but for the attention inside a prompt.
+
+    ``inv_freq`` float64 [rot / 2] and ``scale`` as ``attn_ops.rotary_inv_freq`` returns them (None: no rotation);
+    ``q_weight`` / ``k_weight`` [head_dim]: RMS norms of the heads in front of it.  ``window``: keys that a token sees."""
+
+    def __init__(self, cache, layer, inv_freq=None, *, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, scale=1.0,
+                 softmax_scale=None, window=0):
+        self.cache, self.layer = cache, layer
+        self.k, self.v = cache.k[layer], cache.v[layer]
+        self.inv_freq = None if inv_freq is None else inv_freq.to(self.k.device)
+        self.q_weight, self.k_weight = q_weight, k_weight
+        self.rotary = dict(eps=eps, interleaved=interleaved, scale=scale)
+        self.softmax_scale, self.window = softmax_scale, window
+
+    def prefill(self, q, k, v, positions, seq_ids):
+        """Tokens of one or several prompts, q [T, Hq, D], k and v [T, H, D], with what ``cache.extend`` returned for them.
+        Stores keys and values; returns the queries and keys, turned, for the attention inside the prompt."""
+        from . import attn_ops
+
+        if self.inv_freq is not None:
+            q, k = attn_ops.qk_norm_rotary(q, k, positions, self.inv_freq, self.q_weight, self.k_weight, **self.rotary)
+        elif self.q_weight is not None or self.k_weight is not None:
+            none = torch.empty(0, device=k.device, dtype=torch.float64)
+            q, k = attn_ops.qk_norm_rotary(q, k, positions, none, self.q_weight, self.k_weight, **self.rotary)
+        attn_ops.rotary_append(q[:, :0], k, v, positions, self.k, self.v, self.cache.block_table, seq_ids=seq_ids)
+        return q, k
+
+    def decode(self, q, k, v):
+        """One new token of every row of the cache, q [rows, Hq, D], k and v [rows, H, D], after ``cache.step``: stores its key
+        and value and attends to the row's keys; rows without a sequence (or that ``step`` left out) give zeros.  Two calls,
+        three launches, no allocation but the outputs: can be captured and replayed."""
+        from . import attn_ops
+
+        c = self.cache
+        q = attn_ops.rotary_append(q, k, v, c.positions, self.k, self.v, c.block_table, self.inv_freq, self.q_weight,
+                                   self.k_weight, **self.rotary)
+        return attn_ops.paged_decode_attention(q, self.k, self.v, c.block_table, c.lengths, softmax_scale=self.softmax_scale,
+                                               window=self.window)
