@@ -173,8 +173,65 @@ def test_rotary_one_gradient_wanted_and_unused_output(A):
     (dq,) = torch.autograd.grad(qo.sum(), q)
     back = A.qk_norm_rotary(torch.ones_like(q), None, -pos, freqs(32))
     assert torch.equal(dq, back)
+    w = torch.ones(32, device="cuda", requires_grad=True)
+    qo, ko = A.qk_norm_rotary(q.detach(), k, pos, freqs(32), None, w)
+    (dw,) = torch.autograd.grad(qo.sum(), w)               # the queries do not pass through the keys' weight
+    assert not bool(dw.any())
     with torch.no_grad():
         assert not A.qk_norm_rotary(q, k, pos, freqs(32))[0].requires_grad
+
+
+def test_rotary_gradients_accumulate_into_leaves_and_through_a_graph(A):
+    """backward() into .grad, twice through one graph, outputs changed in place, and gradients on a side stream."""
+    g = gen(30)
+    x = torch.randn(6, 3, 64, generator=g, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    pos, fr = torch.arange(6, device="cuda"), freqs(64)
+    y = A.qk_norm_rotary(2 * x, None, pos, fr, w)
+    z = (y * y).sum()
+    z.backward(retain_graph=True)
+    once = x.grad.clone(), w.grad.clone()
+    z.backward()
+    assert torch.equal(x.grad, 2 * once[0]) and torch.equal(w.grad, 2 * once[1])
+    y = A.qk_norm_rotary(x, None, pos, fr, w)
+    y.mul_(3.0)
+    d1 = torch.autograd.grad(y.sum(), x)[0]
+    d2 = torch.autograd.grad(A.qk_norm_rotary(x, None, pos, fr, w), x, torch.full_like(x, 3.0))[0]
+    assert torch.equal(d1, d2)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        x2, w2 = x.detach().requires_grad_(), w.detach().requires_grad_()
+        d3 = torch.autograd.grad(A.qk_norm_rotary(x2, None, pos, fr, w2), x2, torch.full_like(x, 3.0))[0]
+    s.synchronize()
+    assert torch.equal(d3, d2)
+    y = A.qk_norm_rotary(x, None, pos, fr, w)
+    with torch.no_grad():
+        w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_rotary_training_step_captured_into_a_graph(A):
+    """Forward and backward through autograd inside a capture, replayed on other values."""
+    g = gen(31)
+    x = torch.randn(20, 4, 64, generator=g, device="cuda").bfloat16().requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    pos, fr = torch.arange(20, device="cuda"), freqs(64)
+    dy = torch.randn(20, 4, 64, generator=g, device="cuda").bfloat16()
+    step = lambda: torch.autograd.grad(A.qk_norm_rotary(x, None, pos, fr, w), [x, w], dy)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = step()
+    with torch.no_grad():
+        x.copy_(torch.randn(20, 4, 64, generator=g, device="cuda"))
+    gr.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
 # ------------------------------------------------------------------ cache
@@ -617,7 +674,8 @@ def test_refusals(A):
     refused(TypeError, "host data", A.copy_pages, [pages], pos[:1], [1])
     q = x.clone().requires_grad_()
     g1 = torch.autograd.grad(R_(q, None, pos, fr, w).sum(), q, create_graph=True)[0]
-    refused(RuntimeError, "does not require grad", lambda: torch.autograd.grad(g1.sum(), q))
+    refused(RuntimeError, "not have been used", lambda: torch.autograd.grad(g1.sum(), q, retain_graph=True))
+    refused(RuntimeError, "differentiated once", lambda: g1.sum().backward())
 
 
 # ------------------------------------------------------------------ a run of them together

@@ -15,7 +15,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -56,26 +55,6 @@ def rotary_inv_freq(dim, base=10000.0, *, scaling=None, factor=1.0, trained_leng
     return freq.to(device) if device is not None else freq, scale
 
 
-class QkNormRotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, scale):
-        ctx.args = dict(eps=eps, interleaved=interleaved, scale=scale)
-        ctx.norm = q_weight is not None or k_weight is not None
-        # (a rotation alone is its own inverse's transpose: its gradient needs neither q nor k)
-        ctx.save_for_backward(q if ctx.norm else None, k if ctx.norm else None, positions, inv_freq, q_weight, k_weight)
-        qo, ko = ops.qk_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, **ctx.args)
-        return qo if ko is None else (qo, ko)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk=None):
-        q, k, positions, inv_freq, qw, kw = ctx.saved_tensors
-        if not ctx.norm:
-            q, k = dq, dk
-        gq, gk, gqw, gkw = ops.qk_norm_rotary_bwd(dq, dk, q, k, positions, inv_freq, qw, kw, **ctx.args)
-        return gq, gk, None, None, gqw, gkw, None, None, None
-
-
 def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, eps=1e-6, interleaved=False, scale=1.0):
     """Queries ``q`` [T, Hq, D] or [B, L, Hq, D] and keys ``k`` [.., Hk, D] (or None) -> new tensors of their shapes (only
     the first without ``k``).
@@ -86,11 +65,6 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, e
     int32 or int64, [T], [B, L] or [L] for every batch element; ``inv_freq`` float64 (or float32) on the device, see
     ``rotary_inv_freq``.  Angles are formed in 64 bits, the rest in fp32, rounded once.  Differentiable in q, k and the
     weights (once); the weights' gradients are summed in a fixed order.  D <= 512."""
-    # (spelled out: a generator over the four costs 2 us, a quarter of a small call)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad) or
-                                    (q_weight is not None and q_weight.requires_grad) or
-                                    (k_weight is not None and k_weight.requires_grad)):
-        return QkNormRotary.apply(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, scale)
     qo, ko = ops.qk_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, eps=eps, interleaved=interleaved, scale=scale)
     return qo if k is None else (qo, ko)
 
