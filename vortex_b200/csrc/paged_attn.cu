@@ -558,9 +558,11 @@ template <typename T, bool VEC> __device__ __forceinline__ float4 load4(const T*
     return r;
 }
 
+constexpr int any_blocks_per_sm(int DP, int HP) { return DP == 256 ? (HP == 1 ? 3 : 2) : 4; }
+
 template <typename T, int DP, int HP, bool VEC>
-__global__ void __launch_bounds__(kThreads) decode_any_kernel(const __grid_constant__ AttnArgs a) {
-    constexpr int C = DP / 32, PITCH = DP + 4, STEPS = DP <= 128 ? 2 : 1;
+__global__ void __launch_bounds__(kThreads, any_blocks_per_sm(DP, HP)) decode_any_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int C = DP / 32, PITCH = DP + 4, STEPS = HP == 1 ? 256 / DP : DP == 64 ? 2 : 1;
     __shared__ __align__(16) float s_o[kWarps * HP * PITCH], s_q[HP * DP];
     __shared__ float s_m[kWarps][HP], s_l[kWarps][HP];
     asm volatile("griddepcontrol.launch_dependents;");
@@ -746,7 +748,7 @@ Plan make_plan(const vtx_paged_decode_params& p) {
         per_sm = decode_blocks_per_sm(pl.DP, NT);
     } else {
         pl.HP = G > 1 ? 4 : 1;
-        per_sm = 3;
+        per_sm = any_blocks_per_sm(pl.DP, pl.HP);
     }
     // no more blocks than units
     const int64_t keys = p.block_table ? p.table_width * p.page_size : p.page_size;
