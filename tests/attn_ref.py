@@ -75,9 +75,10 @@ def attend(q, k_pages, v_pages, table, lengths, softmax_scale, window=0):
         out[b] = torch.einsum("hn,nhd->hd", p, v)
         lse[b] = torch.logsumexp(s, -1)
         # a score: D products summed (2 u a step in the tensor cores), scaled, subtracted (|s| 4 u), exponential (2 ulp): an
-        # error of a probability in both sums; the probability as head and remainder (2^-17); the sums over the keys of a
-        # warp, its lanes, warps and blocks
+        # error of a probability in both sums; the probability as head and remainder: a head of 8 bits towards zero leaves less
+        # than 2^-7 of it, which is rounded to 8 bits (2^-9 of it), so 2^-16; the sums over the keys of a warp, its lanes,
+        # warps and blocks
         mag = torch.einsum("hd,nhd->hn", qb.abs(), k.abs()).amax(-1)
-        c = 2 * ((2 * D + 8) * U * mag + 8 * U) + 2.0 ** -17 + 2 * U * (len(range(lo, n)) / 16 + 64)
+        c = 2 * ((2 * D + 8) * U * mag + 8 * U) + 2.0 ** -16 + 2 * U * (len(range(lo, n)) / 16 + 64)
         bound[b] = c[:, None] * torch.einsum("hn,nhd->hd", p, v.abs())
     return out, lse, bound

@@ -406,8 +406,27 @@ def test_decode_attention_many_light_keys_beside_a_heavy_one(A, io, Hq):
         w = (n - 1) * 2.0 ** -25
         ref = torch.full((1, Hq, D), 64.0 * w / (1 + w), dtype=torch.float64, device="cuda")
         # exact products and powers of two but for the scale's rounding (25 u of the exponent) and n / 64 sums a warp
-        tol = R.rounding(ref, dt) + (2.0 ** -17 + (2 * 25 + n / 64 + 64) * 2 * R.U) * ref
+        tol = R.rounding(ref, dt) + (2.0 ** -16 + (2 * 25 + n / 64 + 64) * 2 * R.U) * ref
         within(out, ref, tol, f"heavy key {at}")
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16", "f32"])
+def test_decode_attention_infinite_values_come_out_as_they_are(A, io):
+    """At the heaviest key, whose probability is a power of two, at keys of any other weight, with either sign; both signs in a
+    column, or a NaN, give NaN."""
+    dt, D, n = DT[io], 64, 200
+    g = gen(23)
+    q, k, v = (torch.randn(1, m, h, D, generator=g, device="cuda").to(dt) for m, h in ((1, 2), (n, 1), (n, 1)))
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    top = torch.einsum("hd,nd->hn", q[0, 0].float(), k[0, :, 0].float()).argmax(-1)
+    v[0, top[0], 0, 0] = float("inf")
+    v[0, top[1], 0, 1] = float("-inf")
+    for j in range(0, n, 3):
+        v[0, j, 0, 2 + j % 20] = float("inf")
+    v[0, 3, 0, 30], v[0, 4, 0, 30], v[0, 9, 0, 31] = float("inf"), float("-inf"), float("nan")
+    out = A.paged_decode_attention(q[0], k, v, None, lens)
+    ref, _, _ = R.attend(q[0], k, v, None, [n], D ** -0.5)
+    assert torch.equal(out.isnan(), ref.isnan()) and torch.equal(out.isposinf(), ref.isposinf()) and torch.equal(out.isneginf(), ref.isneginf())
 
 
 def test_decode_attention_far_apart_scores(A):

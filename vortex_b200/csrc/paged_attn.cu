@@ -24,6 +24,7 @@
 
 #include "attn.cuh"
 #include "tma.cuh"
+#include "umma.cuh"
 
 VTX_DEFINE_STATUS_READER()
 
@@ -85,7 +86,7 @@ struct Seq {                        // keys lo .. n-1 of a sequence; tiles start
         lo = (len > a.window) ? len - a.window : 0;
         if (lo > n) lo = n;
         base = lo & ~(kTile - 1);
-        units = n > base ? (n - base + a.unit - 1) / a.unit : 1;      // an empty one has a unit, to write its zeros
+        units = n > base ? (int)(((unsigned)(n - base) + a.unit - 1) / a.unit) : 1;      // an empty one has a unit, to write its zeros
     }
 };
 
@@ -258,13 +259,25 @@ __device__ __forceinline__ uint4 ld16(const void* p) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    T t[2] = {from_f32<T>(lo), from_f32<T>(hi)};
-    return *reinterpret_cast<uint32_t*>(t);
+// Two probabilities p, q >= 0 as heads and remainders of the I/O type, packed: the head towards zero, so that no remainder is
+// negative, and no remainder of a probability above the type's smallest step is zero: a value of infinity then comes out as
+// infinity, not as the difference of two or as 0 * inf.  What that adds is below 2^-24 of the largest probability a key in
+// fp16 (p is near 2^11 there), 2^-126 in bf16.  Head and remainder differ from p by at most 2^-16 of it (bf16: the remainder
+// is below 2^-7, rounded to 8 bits).
+template <typename T> __device__ __forceinline__ void split(float p, float q, uint32_t& head, uint32_t& rest);
+template <> __device__ __forceinline__ void split<__nv_bfloat16>(float p, float q, uint32_t& head, uint32_t& rest) {
+    const uint32_t a = __float_as_uint(p), b = __float_as_uint(q);
+    head = __byte_perm(a, b, 0x7632);
+    const float x = p - __uint_as_float(a & 0xffff0000u), y = q - __uint_as_float(b & 0xffff0000u);
+    rest = umma::pack_bf16(p > 0.f ? fmaxf(x, FLT_MIN) : x, q > 0.f ? fmaxf(y, FLT_MIN) : y);
 }
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x) {
-    const T* t = reinterpret_cast<const T*>(&x);
-    return make_float2(to_f32<T>(t[0]), to_f32<T>(t[1]));
+template <> __device__ __forceinline__ void split<__half>(float p, float q, uint32_t& head, uint32_t& rest) {
+    constexpr float step = 5.9604644775390625e-8f;      // 2^-24
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(head) : "f"(q), "f"(p));
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&head));
+    const float x = p - h.x, y = q - h.y;
+    const __half2 r = __floats2half2_rn(p >= step ? fmaxf(x, step) : x, q >= step ? fmaxf(y, step) : y);
+    rest = *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
@@ -488,10 +501,10 @@ __global__ void __launch_bounds__(kThreads, decode_blocks_per_sm(DP, NT)) decode
                         const float p0 = exp2f(s[x][nt][2 * i] - m[nt][0]), p1 = exp2f(s[x][nt][2 * i + 1] - m[nt][1]);
                         l[nt][0] += p0;
                         l[nt][1] += p1;
-                        const uint32_t hi = pack2<T>(p0, p1);
-                        const float2 back = unpack2<T>(hi);
-                        ph[nt][i] = transpose8(hi);
-                        pl[nt][i] = transpose8(pack2<T>(p0 - back.x, p1 - back.y));
+                        uint32_t head, rest;
+                        split<T>(p0, p1, head, rest);
+                        ph[nt][i] = transpose8(head);
+                        pl[nt][i] = transpose8(rest);
                     }
 #pragma unroll
                 for (int i = 0; i < VC; ++i)
@@ -763,6 +776,7 @@ Plan make_plan(const vtx_paged_decode_params& p) {
 }
 
 template <typename T, int DP, int HP> int launch_join(const AttnArgs& a, int W, cudaStream_t s) {
+    if (int rc = check_launch("paged_decode_attention")) return rc;          // (nothing was written that could be joined)
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)W, (unsigned)(a.G < HP ? a.G : HP));
     cfg.blockDim = dim3(kThreads);
@@ -773,7 +787,7 @@ template <typename T, int DP, int HP> int launch_join(const AttnArgs& a, int W, 
     cfg.attrs = at;
     cfg.numAttrs = 1;
     cudaLaunchKernelEx(&cfg, join_kernel<T, DP, HP>, a, W);
-    return check_launch("paged_decode_attention", 2);
+    return check_launch("paged_decode_attention");
 }
 
 template <typename T, int DP> int launch_tensor(const AttnArgs& a, const Plan& pl, cudaStream_t s) {

@@ -718,10 +718,8 @@ extern "C" int vtx_qk_norm_rotary_bwd(const vtx_rotary_bwd_params* p, void* stre
     a.dy[1] = p->dk_out; a.dyb[1] = p->dk_out_stride_b; a.dyl[1] = p->dk_out_stride_l; a.dyh[1] = p->dk_out_stride_h;
     a.dw_part = static_cast<float*>(p->scratch);
     int64_t q_rows = 0, k_rows = 0;
-    long long launches = 1;
     if (tokens && f.Hq + f.Hk) {
         const int lanes = vector_lanes(a, dtype_size(f.io_dtype));
-        launches = 2;
         if (!lanes) {
             const int64_t warps = ceil_div<int64_t>(tokens * (f.Hq + f.Hk), kThreads / 32);
             q_rows = k_rows = warps < kBwdBlocks ? warps : kBwdBlocks;
@@ -743,10 +741,12 @@ extern "C" int vtx_qk_norm_rotary_bwd(const vtx_rotary_bwd_params* p, void* stre
             }));
         }
     }
+    if (q_rows + k_rows)
+        if (int rc = check_launch("qk_norm_rotary_bwd")) return rc;
     rotary_dw_kernel<<<(unsigned)ceil_div<int64_t>(2 * f.D, kThreads / 32), kThreads, 0, s>>>(
         a.dw_part, (int)q_rows, (int)k_rows, (int)f.D, f.q_weight ? p->dq_weight : nullptr, (int)f.q_weight_dtype,
         f.k_weight ? p->dk_weight : nullptr, (int)f.k_weight_dtype);
-    return check_launch("qk_norm_rotary_bwd", launches);
+    return check_launch("qk_norm_rotary_bwd");
 }
 
 extern "C" int vtx_rotary_append(const vtx_rotary_append_params* p, void* stream) {
