@@ -3,7 +3,11 @@
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = exp2(s_j - m),  s_j = log2(e) * softmax_scale * (q . k_j)
 //
 // in one pass over the cache with a running maximum m.  Every key and value is read once for up to 16 query heads, two
-// operations a byte and head: memory bounds it.  What the kernels are built around:
+// operations a byte and head: memory bounds it.  Measured (bf16, of the measured copy bandwidth): 64 sequences of 8192-8704
+// keys, 32 heads of 128, 1285-1320 us and one of 1,048,576 keys, 8 heads, 640-657 us (1.0); 32 sequences of 4000-8000 keys, 64
+// query heads over 8, 126 us (0.95); 48 ragged ones, 32 over 8 heads of 64 in fp16, 233-245 us (0.85-0.89: rows of 128 bytes
+// at a time); one of 700 keys 10.5 us (a chain of launch, lengths, table, keys, join and join's launch).  What the kernels are
+// built around:
 //
 // * Work.  The cache is cut into units of 64 or 128 keys of one key head; the units of all sequences and heads, in a row, are dealt
 //   out to the blocks in equal runs, whatever the lengths (they are on the device: every block sums them up itself).  A run
@@ -315,6 +319,8 @@ template <bool IN_PAGE> struct Tile {
     int64_t krow[2], vrow[4];             // else: offsets of the lane's rows
 };
 
+// As many as the registers allow without spilling in the loop (heads of 128: three 1288 us, two 1450 at 64 x 8192-8704 keys;
+// of 64 in fp16, ragged: four 237, three 241, five 406).
 constexpr int decode_blocks_per_sm(int DP, int NT) { return DP == 64 ? (NT == 1 ? 4 : 3) : DP == 128 ? (NT == 1 ? 3 : 2) : 2; }
 
 template <typename T, int DP, int NT, bool IN_PAGE>
@@ -552,7 +558,9 @@ __global__ void __launch_bounds__(kThreads, decode_blocks_per_sm(DP, NT)) decode
 
 // ---- any type, head size and alignment: fp32 products on the CUDA cores ----------------------------------------------------
 // Eight lanes hold a key, a lane the values 32 i + 4 (lane % 8) .. + 3 of it; a warp works on four keys at a time, each group
-// of eight lanes with a maximum and sums of its own.  Up to four query heads at a time.
+// of eight lanes with a maximum and sums of its own.  Up to four query heads at a time; one alone leaves registers for more
+// keys in flight.  fp32, 16 sequences of 4000-8000 keys, 16 heads of 128: 235 us (1.0); 32 sequences, 32 over 8 heads: 377 us
+// (0.64: issue slots, and one step in flight).
 template <typename T, bool VEC> __device__ __forceinline__ float4 load4(const T* p, int d, int D) {
     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
     if (VEC) {

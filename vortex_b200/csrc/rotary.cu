@@ -7,9 +7,14 @@
 //   backward, with g = the transposed rotation of dy:  dx = (w g - xh mean(w g xh)) / r,  dw = sum over rows of g xh.
 //
 // Every value is read once and written once, in fp32 between the two, rounded once: memory bounds it, and below some 10^4
-// rows the launch.  What is shared is shared: the sine and cosine of a (token, pair) are formed once per block and token, in
-// shared memory, and used by all heads.  The angle is formed in 64 bits, as turns with the whole turns taken off, since
-// position * inv_freq in 32 bits is off by 0.03 rad at position 2^20; what is left goes to sincospif.
+// rows the launch.  The sine and cosine of a (token, pair) are formed once for up to 16 heads, in shared memory.  The angle is
+// formed in 64 bits, as turns with the whole turns taken off, since position * inv_freq in 32 bits is off by 0.03 rad at
+// position 2^20; what is left goes to sincospif.
+//
+// Measured (bf16, heads of 128, of the measured copy bandwidth): 32768 tokens x 64 heads turned in 167 us (0.98); 16384 tokens x
+// 40 heads normed and turned in 68 us (0.75: the norm's two waits for other lanes, and warps of 8 key heads that are short
+// beside their set-up), backward 100 us (0.77: registers, two blocks an SM); 9757 ragged tokens x 48 heads stored in pages in
+// 50 us (0.73); 64 tokens x 64 heads in 2.8 us, stored 3.8 us (the chain position -> table -> store behind the launch).
 #include "attn.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
@@ -202,8 +207,8 @@ template <typename T, bool INTER> struct Lane {
 };
 
 // Values of a head as its lanes hold them, in shared memory: quad q of a lane's at [q][lane], so that the lanes read
-// neighbouring 16 bytes.  Registers are worth more than shared-memory reads here: what hides the memory is the number of warps
-// (the cosines, sines and weights in registers, and loads a step or two ahead: 199 instead of %ROT% us for 32768 tokens x 64 heads).
+// neighbouring 16 bytes.  Not in registers: what hides the memory is the number of warps (five blocks an SM with one step
+// loaded ahead 167 us for 32768 tokens x 64 heads; cosines and sines in registers, three blocks and two steps 199).
 template <int LANES> __device__ __forceinline__ void load_quad(const float* w, int q, int sub, f32x2& w0, f32x2& w1) {
     const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(w + (q * LANES + sub) * 4);
     w0 = v.x;
@@ -578,24 +583,27 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rotary_bwd_any
     }
 }
 
-// Partial sums, q_rows rows of D for the queries and k_rows for the keys, -> the two weight gradients in the weights' types.  A
-// warp per value.
-__global__ void __launch_bounds__(kThreads) rotary_dw_kernel(const float* part, int q_rows, int k_rows, int D, void* dwq, int qd, void* dwk, int kd) {
-    const int i = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (i >= 2 * D) return;
-    const bool key = i >= D;
+// Partial sums, q_rows rows of D for the queries and k_rows for the keys, -> the two weight gradients in the weights' types.
+// Block (x, which): 32 values, 32 rows of them at a time.  (A warp per value read 32 lines for 32 numbers: 6.9 us.)
+__global__ void __launch_bounds__(1024) rotary_dw_kernel(const float* part, int q_rows, int k_rows, int D, void* dwq, int qd, void* dwk, int kd) {
+    __shared__ float s_sum[32][33];
+    const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, at = blockIdx.x * 32 + lane, key = blockIdx.y;
     void* out = key ? dwk : dwq;
     if (!out) return;
-    const int at = key ? i - D : i, rows = key ? k_rows : q_rows;
-    const float* p = part + (key ? (int64_t)q_rows * D : 0) + at;
+    const int rows = key ? k_rows : q_rows, code = key ? kd : qd;
+    const float* p = part + (key ? (int64_t)q_rows * D : 0);
     float s = 0.f;
-    for (int b = lane; b < rows; b += 32) s += p[(int64_t)b * D];
-    s = group_sum<32>(s);
-    if (lane) return;
-    const int code = key ? kd : qd;
-    if (code == VTX_F32) static_cast<float*>(out)[at] = s;
-    else if (code == VTX_BF16) static_cast<__nv_bfloat16*>(out)[at] = from_f32<__nv_bfloat16>(s);
-    else static_cast<__half*>(out)[at] = from_f32<__half>(s);
+    if (at < D)
+#pragma unroll 4
+        for (int b = row; b < rows; b += 32) s += p[(int64_t)b * D + at];
+    s_sum[row][lane] = s;
+    __syncthreads();
+    s = group_sum<32>(s_sum[lane][row]);                           // (warp `row` now holds one value's 32 sums)
+    const int i = blockIdx.x * 32 + row;
+    if (lane || i >= D) return;
+    if (code == VTX_F32) static_cast<float*>(out)[i] = s;
+    else if (code == VTX_BF16) static_cast<__nv_bfloat16*>(out)[i] = from_f32<__nv_bfloat16>(s);
+    else static_cast<__half*>(out)[i] = from_f32<__half>(s);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -743,7 +751,7 @@ extern "C" int vtx_qk_norm_rotary_bwd(const vtx_rotary_bwd_params* p, void* stre
     }
     if (q_rows + k_rows)
         if (int rc = check_launch("qk_norm_rotary_bwd")) return rc;
-    rotary_dw_kernel<<<(unsigned)ceil_div<int64_t>(2 * f.D, kThreads / 32), kThreads, 0, s>>>(
+    rotary_dw_kernel<<<dim3((unsigned)ceil_div<int64_t>(f.D, 32), 2), 1024, 0, s>>>(
         a.dw_part, (int)q_rows, (int)k_rows, (int)f.D, f.q_weight ? p->dq_weight : nullptr, (int)f.q_weight_dtype,
         f.k_weight ? p->dk_weight : nullptr, (int)f.k_weight_dtype);
     return check_launch("qk_norm_rotary_bwd");
