@@ -250,7 +250,12 @@ def host():
         if mod.abi_version() != header_abi_version():
             raise RuntimeError(f"{HOST_PATH} was built for ABI version {mod.abi_version()}: rebuild it with "
                                "`python -m vortex_b200.build`")
-        mod.bind({n: C.cast(getattr(handle, n), _p).value for n in SYMBOLS})
+        address = lambda n: C.cast(getattr(handle, n), _p).value  # noqa: E731
+        mod.bind(*(address(n) for n in ("vtx_decode_layer", "vtx_fused_fir_fwd", "vtx_fused_iir_fwd", "vtx_fused_iir_scratch_bytes",
+                                        "vtx_last_error")))
+        mod.bind_attention({n: address(n) for n in ("vtx_qk_norm_rotary_fwd", "vtx_qk_norm_rotary_bwd", "vtx_qk_norm_rotary_bwd_scratch_bytes",
+                                                    "vtx_rotary_append", "vtx_paged_decode_attention", "vtx_paged_decode_scratch_bytes",
+                                                    "vtx_copy_pages")})
         _host = mod
     return _host
 

@@ -558,13 +558,15 @@ void copy_pages(const std::vector<Tensor>& pools, const std::vector<int64_t>& sr
 
 PYBIND11_MODULE(_vtx_host, m) {
     m.def("abi_version", [] { return VTX_ABI_VERSION; });
-    // addresses of the library's functions by name; all that this module calls must be among them
-    m.def("bind", [](const std::map<std::string, uintptr_t>& f) {
-        p_decode_layer = reinterpret_cast<decltype(p_decode_layer)>(f.at("vtx_decode_layer"));
-        p_fused_fir_fwd = reinterpret_cast<decltype(p_fused_fir_fwd)>(f.at("vtx_fused_fir_fwd"));
-        p_fused_iir_fwd = reinterpret_cast<decltype(p_fused_iir_fwd)>(f.at("vtx_fused_iir_fwd"));
-        p_fused_iir_scratch_bytes = reinterpret_cast<decltype(p_fused_iir_scratch_bytes)>(f.at("vtx_fused_iir_scratch_bytes"));
-        p_last_error = reinterpret_cast<decltype(p_last_error)>(f.at("vtx_last_error"));
+    m.def("bind", [](uintptr_t decode, uintptr_t fir, uintptr_t iir, uintptr_t iir_scratch, uintptr_t last_error) {
+        p_decode_layer = reinterpret_cast<decltype(p_decode_layer)>(decode);
+        p_fused_fir_fwd = reinterpret_cast<decltype(p_fused_fir_fwd)>(fir);
+        p_fused_iir_fwd = reinterpret_cast<decltype(p_fused_iir_fwd)>(iir);
+        p_fused_iir_scratch_bytes = reinterpret_cast<decltype(p_fused_iir_scratch_bytes)>(iir_scratch);
+        p_last_error = reinterpret_cast<decltype(p_last_error)>(last_error);
+    });
+    // the attention layers' functions, by name
+    m.def("bind_attention", [](const std::map<std::string, uintptr_t>& f) {
         p_rotary_fwd = reinterpret_cast<decltype(p_rotary_fwd)>(f.at("vtx_qk_norm_rotary_fwd"));
         p_rotary_bwd = reinterpret_cast<decltype(p_rotary_bwd)>(f.at("vtx_qk_norm_rotary_bwd"));
         p_rotary_bwd_scratch_bytes = reinterpret_cast<decltype(p_rotary_bwd_scratch_bytes)>(f.at("vtx_qk_norm_rotary_bwd_scratch_bytes"));
