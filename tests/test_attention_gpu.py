@@ -488,6 +488,23 @@ def test_decode_attention_many_sequences(A, io, page):
     within(out, ref, bound + R.rounding(ref.abs() + bound, dt), "out")
 
 
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("Hq,Hk,D", [(32, 32, 128), (600, 600, 64), (45, 15, 128), (14, 7, 80), (20, 20, 40), (74, 2, 64)])
+def test_decode_attention_work_dealt_out(A, io, Hq, Hk, D):
+    """Enough keys for every block of the machine: heads abreast or in a row, more heads than blocks, runs that end anywhere."""
+    g, dt = gen(24), DT[io]
+    for lengths in ([3000], [1500, 3, 0, 700], [257] * 9, [5000, 1, 1, 1]):
+        table, n = make_table(g, lengths, 16)
+        kp, vp = pools(g, n, 16, Hk, D, dt)
+        q = torch.randn(len(lengths), Hq, D, generator=g, device="cuda").to(dt)
+        out, lse = A.paged_decode_attention(q, kp, vp, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), return_lse=True)
+        ref, lref, bound = R.attend(q, kp, vp, table, lengths, D ** -0.5)
+        within(out, ref, bound + R.rounding(ref.abs() + bound, dt), str(lengths))
+        full = lref > float("-inf")
+        # a score: (2 D + 8) u sum |q k| scale, at most 264 u 40 = 6e-4; the sum and its logarithm 1e-4
+        assert torch.equal(lse > float("-inf"), full) and float((lse - lref)[full].abs().max()) < 1e-3
+
+
 def test_decode_attention_offsets_beyond_32_bits(A):
     """A pool of more than 2^31 values (2^32 bytes): keys in its last pages."""
     D, page, n = 128, 256, (1 << 17) + 3

@@ -4,22 +4,22 @@
 //
 // in one pass over the cache with a running maximum m.  Every key and value is read once for up to 16 query heads, two
 // operations a byte and head: memory bounds it.  Measured (bf16, of the measured copy bandwidth): 64 sequences of 8192-8704
-// keys, 32 heads of 128, 1285-1320 us and one of 1,048,576 keys, 8 heads, 640-657 us (1.0); 32 sequences of 4000-8000 keys, 64
-// query heads over 8, 126 us (0.95); 48 ragged ones, 32 over 8 heads of 64 in fp16, 233-245 us (0.85-0.89: rows of 128 bytes
-// at a time); one of 700 keys 10.5 us (a chain of launch, lengths, table, keys, join and join's launch).  What the kernels are
-// built around:
+// keys, 32 heads of 128, 1285-1320 us and one of 1,048,576 keys, 8 heads, 631 us (1.0); 32 sequences of 4000-8000 keys, 64
+// query heads over 8, 126-130 us (0.95); 48 ragged ones, 32 over 8 heads of 64 in fp16, 224 us (0.93); one of 700 keys 9.8 us
+// (a chain of launch, lengths, table, keys, join and join's launch).  What the kernels are built around:
 //
-// * Work.  The cache is cut into units of 64 or 128 keys of one key head; the units of all sequences and heads, in a row, are dealt
-//   out to the blocks in equal runs, whatever the lengths (they are on the device: every block sums them up itself).  A run
-//   covers the end of one (sequence, head), some whole ones, and the beginning of another; whole ones are finished in place,
-//   the two open ones leave (m, sum, unnormalised out) in the scratch, which the second kernel joins.  At most two open ones a
-//   block: the scratch does not grow with the batch.  Launched so that it is set up while the first kernel still runs.
+// * Work.  The cache is cut into units of 64 or 128 keys of one key head; the units of all sequences, in a row, are dealt out in
+//   equal runs, whatever the lengths (they are on the device: every block sums them up itself), a run to a block for each head,
+//   or, with the heads' units in the row as well, to one block (make_plan chooses).  A block's run covers the end of one
+//   (sequence, head), some whole ones, and the beginning of another; whole ones are finished in place, the two open ones leave
+//   (m, sum, unnormalised out) in the scratch, which the second kernel joins.  At most two open ones a block: the scratch does
+//   not grow with the batch.  The second kernel is launched so that it is set up while the first still runs.
 // * No shared memory on the way.  With keys as the rows of the first product (S^T = K Q^T) a lane's piece of the A operand is
 //   16 contiguous bytes of two key rows, once the order of the summed dimensions is agreed with Q; for the second
 //   (O^T = V^T P^T) it is 16 contiguous bytes of four value rows, after one byte permutation a register.  So loads go from
 //   global memory to the registers that the mma.sync reads; 16 keys are 16 loads of 16 bytes a lane, the next tile's keys are
 //   in flight from the moment the scores exist, its values from the moment the second product is issued.  Tensor cores at
-//   16 x 8 x 16 are enough: even with one query head of eight columns they are under a tenth busy.
+//   16 x 8 x 16 are enough: with one query head of eight columns used their pipe is 15 % busy.
 // * P is brought from the accumulator's layout to the B operand's by transposing 8 x 8 blocks (movmatrix), as head and
 //   remainder: rounded to bf16 alone it would cost as much as the output's own rounding.
 // * The maximum is raised only when a score passes it by more than a slack (2^8, for fp16 2^4): most tiles then need neither
@@ -69,13 +69,14 @@ struct AttnArgs {
     int B, Hq, G, D, page_size, num_pages;
     int passes, head_groups;        // passes over the G query heads of a key head; Hk * passes
     int unit;                       // keys of a unit of work
+    int abreast;                    // head groups whose blocks walk the same keys side by side (1, or all of them)
     int64_t max_keys;
 };
 
-// The (sequence, head group) that begins in a block's run and ends in the run of block `last`.
+// The (sequence, head group) that begins in a block's run and ends in the `runs`-th run from there.
 struct Open {
-    int64_t units;                  // of the whole call
-    int b, hg, last, pad;
+    int64_t units;                  // of all runs
+    int b, hg, runs, pad;
 };
 
 struct Seq {                        // keys lo .. n-1 of a sequence; tiles start at lo & ~15
@@ -123,36 +124,40 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_tot, int64_t
 // The block's run of units and the sequence in which it starts.
 struct Run {
     int64_t units, at, end, seq_first;     // of all; next, end; first unit of sequence b
-    int b;
+    int b, hg0, inner, run, runs;          // sequence; the block's head group, or the first; head groups in the run; run of runs
     __device__ Run(const AttnArgs& a) {
         __shared__ int64_t s_tot[kWarps], s_first;
         __shared__ int s_b;
         const int tid = threadIdx.x;
+        inner = a.head_groups / a.abreast;
+        run = blockIdx.x / a.abreast;
+        runs = gridDim.x / a.abreast;
+        hg0 = blockIdx.x - run * a.abreast;
         if (a.B <= 32) {                    // every warp for itself
             const int lane = tid & 31;
-            const int64_t own = lane < a.B ? (int64_t)Seq(a, lane).units * a.head_groups : 0, incl = warp_scan(own);
+            const int64_t own = lane < a.B ? (int64_t)Seq(a, lane).units * inner : 0, incl = warp_scan(own);
             units = __shfl_sync(0xffffffffu, incl, 31);
-            at = run_start(units, blockIdx.x, gridDim.x);
-            end = run_start(units, blockIdx.x + 1, gridDim.x);
+            at = run_start(units, run, runs);
+            end = run_start(units, run + 1, runs);
             const unsigned in = __ballot_sync(0xffffffffu, at >= incl - own && at < incl);
             b = in ? __ffs(in) - 1 : 0;
             seq_first = __shfl_sync(0xffffffffu, incl - own, b);
             return;
         }
-        int64_t mine = tid < a.B ? (int64_t)Seq(a, tid).units * a.head_groups : 0, total, incl;
+        int64_t mine = tid < a.B ? (int64_t)Seq(a, tid).units * inner : 0, total, incl;
         incl = block_scan(mine, s_tot, total);
         units = total;
         for (int c = kThreads; c < a.B; c += kThreads) {
             int64_t t;
-            block_scan(c + tid < a.B ? (int64_t)Seq(a, c + tid).units * a.head_groups : 0, s_tot, t);
+            block_scan(c + tid < a.B ? (int64_t)Seq(a, c + tid).units * inner : 0, s_tot, t);
             units += t;
         }
-        at = run_start(units, blockIdx.x, gridDim.x);
-        end = run_start(units, blockIdx.x + 1, gridDim.x);
+        at = run_start(units, run, runs);
+        end = run_start(units, run + 1, runs);
         int64_t before = 0;
         for (int c = 0;; c += kThreads) {
             if (c) {
-                mine = c + tid < a.B ? (int64_t)Seq(a, c + tid).units * a.head_groups : 0;
+                mine = c + tid < a.B ? (int64_t)Seq(a, c + tid).units * inner : 0;
                 incl = block_scan(mine, s_tot, total);
             }
             if (at < before + total || c + kThreads >= a.B) {
@@ -179,8 +184,9 @@ template <int HP> __device__ __forceinline__ Piece next_piece(const AttnArgs& a,
     Piece p;
     p.b = r.b; p.units = s.units; p.lo = s.lo; p.n = s.n; p.base = s.base;
     const int64_t in = r.at - r.seq_first;
-    p.hg = (int)(in / s.units);
-    p.c0 = (int)(in - (int64_t)p.hg * s.units);
+    const int hg = (int)(in / s.units);
+    p.hg = r.hg0 + hg;
+    p.c0 = (int)(in - (int64_t)hg * s.units);
     const int64_t left = r.end - r.at;
     p.c1 = (int)(p.c0 + left < s.units ? p.c0 + left : s.units);
     p.kvh = p.hg / a.passes;
@@ -188,8 +194,8 @@ template <int HP> __device__ __forceinline__ Piece next_piece(const AttnArgs& a,
     p.h0 = p.kvh * a.G + first;
     p.heads = a.G - first < HP ? a.G - first : HP;
     r.at += p.c1 - p.c0;
-    if (p.hg == a.head_groups - 1 && p.c1 == s.units) {
-        r.seq_first += (int64_t)s.units * a.head_groups;
+    if (hg == r.inner - 1 && p.c1 == s.units) {
+        r.seq_first += (int64_t)s.units * r.inner;
         ++r.b;
     }
     return p;
@@ -236,10 +242,10 @@ __device__ __forceinline__ void join_warps(const AttnArgs& a, const Piece& p, co
     }
     if (threadIdx.x == 0 && p.c0 == 0 && !whole) {
         const int64_t last_unit = r.at - p.c1 + p.units - 1;        // (r.at is behind this piece)
-        int w = (int)(last_unit * gridDim.x / r.units);
-        while (w + 1 < (int)gridDim.x && run_start(r.units, w + 1, gridDim.x) <= last_unit) ++w;
-        while (run_start(r.units, w, gridDim.x) > last_unit) --w;
-        a.open[blockIdx.x] = Open{r.units, p.b, p.hg, w, 0};
+        int w = (int)(last_unit * r.runs / r.units);
+        while (w + 1 < r.runs && run_start(r.units, w + 1, r.runs) <= last_unit) ++w;
+        while (run_start(r.units, w, r.runs) > last_unit) --w;
+        a.open[blockIdx.x] = Open{r.units, p.b, p.hg, w - r.run + 1, 0};
     }
 }
 
@@ -559,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, decode_blocks_per_sm(DP, NT)) decode
 // ---- any type, head size and alignment: fp32 products on the CUDA cores ----------------------------------------------------
 // Eight lanes hold a key, a lane the values 32 i + 4 (lane % 8) .. + 3 of it; a warp works on four keys at a time, each group
 // of eight lanes with a maximum and sums of its own.  Up to four query heads at a time; one alone leaves registers for more
-// keys in flight.  fp32, 16 sequences of 4000-8000 keys, 16 heads of 128: 235 us (1.0); 32 sequences, 32 over 8 heads: 377 us
+// keys in flight.  fp32, 16 sequences of 4000-8000 keys, 16 heads of 128: 228 us (1.0); 32 sequences, 32 over 8 heads: 373 us
 // (0.64: issue slots, and one step in flight).
 template <typename T, bool VEC> __device__ __forceinline__ float4 load4(const T* p, int d, int D) {
     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -704,11 +710,11 @@ template <typename T, int DP, int HP> __global__ void __launch_bounds__(kThreads
     if (op.b < 0) return;
     const int kvh = op.hg / a.passes, first = (op.hg - kvh * a.passes) * HP;
     if (first + h >= a.G) return;
-    const int n = op.last - w0 + 1;
+    const int n = op.runs, run0 = w0 / a.abreast, runs = W / a.abreast;
     // the run it begins in keeps it in slot 1, the others in slot 0; a run may be empty
-    auto row = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i == 0)) * HP + h; };
-    const bool sparse = op.units < W;
-    auto empty = [&](int i) { return run_start(op.units, w0 + i, W) == run_start(op.units, w0 + i + 1, W); };
+    auto row = [&](int i) { return ((int64_t)(w0 + i * a.abreast) * 2 + (i == 0)) * HP + h; };
+    const bool sparse = op.units < runs;
+    auto empty = [&](int i) { return run_start(op.units, run0 + i, runs) == run_start(op.units, run0 + i + 1, runs); };
     const int q = tid % Q, r0 = tid / Q;
     float m = -FLT_MAX, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -741,7 +747,7 @@ template <typename T, int DP, int HP> __global__ void __launch_bounds__(kThreads
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
 struct Plan {
-    int DP, HP, blocks, unit;
+    int DP, HP, blocks, unit, abreast;
     bool tensor, in_page, vec;
     int64_t slots, bytes;
 };
@@ -778,6 +784,15 @@ Plan make_plan(const vtx_paged_decode_params& p) {
     const int64_t pairs = p.B * p.Hk * ceil_div<int64_t>(G, pl.HP);
     int64_t most = pairs > (1 << 20) ? pairs : pairs * (per_seq > 0 ? per_seq : 1);
     pl.blocks = (int)(most < (int64_t)kNumSMs * per_sm ? most : (int64_t)kNumSMs * per_sm);
+    const int64_t groups = p.Hk * ceil_div<int64_t>(G, pl.HP);
+    // Head groups abreast -- the blocks of a run walk the same keys of all heads side by side, whose rows are neighbours in
+    // memory -- where that leaves no more than a twentieth of the blocks out, or where rows share 128-byte lines, which DRAM
+    // delivers whole.  Else all heads' units in one row.  (us abreast / in a row: 1,048,576 keys x 8 heads 631 / 651, ragged 8
+    // heads of 64 224 / 248, 256 sequences of 100-600 keys 76 / 81, 16 heads of 112 262 / 297, of 80 234 / 252; 64 x 8192-8704
+    // keys x 32 heads, 416 of 444 blocks, 1325 / 1306.)
+    const bool lines = (p.D * es) % 128 == 0;
+    pl.abreast = groups <= pl.blocks && (pl.blocks % groups * 20 <= pl.blocks || !lines) ? (int)groups : 1;
+    pl.blocks -= pl.blocks % pl.abreast;
     pl.slots = (int64_t)pl.blocks * 2 * pl.HP;
     pl.bytes = pl.slots * (pl.DP * 4 + 8) + (int64_t)pl.blocks * sizeof(Open);
     return pl;
@@ -874,6 +889,7 @@ extern "C" int vtx_paged_decode_attention(const vtx_paged_decode_params* p, void
     a.page_size = (int)p->page_size; a.num_pages = (int)p->num_pages;
     a.passes = (a.G + pl.HP - 1) / pl.HP;
     a.unit = pl.unit;
+    a.abreast = pl.abreast;
     a.head_groups = (int)p->Hk * a.passes;
     a.max_keys = p->block_table ? p->table_width * p->page_size : p->page_size;
     cudaStream_t s = (cudaStream_t)stream;
