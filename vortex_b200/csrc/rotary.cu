@@ -76,20 +76,37 @@ __device__ __forceinline__ float2 turn(const RotArgs& a, int64_t pos, int i) {
     return make_float2(c * a.scale, (a.conj ? -s : s) * a.scale);
 }
 
-// Element offset of a token's row in the pages of the k (which = 1) or v (2) pool, or -1 where the token is not stored: a
-// negative position is padding; one behind its table row, or a page outside the pool, sets the status word.
-__device__ __forceinline__ int64_t slot_offset(const RotArgs& a, int64_t tok, int64_t pos, int which) {
-    if (pos < 0) return -1;
-    const int64_t seq = a.seq_ids ? (int64_t)a.seq_ids[tok] : tok;
-    const int64_t at = pos / a.page_size;
-    int64_t page = -1;
-    if (seq >= 0 && seq < a.num_seqs && at < a.table_width) page = a.table[seq * a.table_stride + at];
-    if (page < 0 || page >= a.num_pages) {
-        atomicCAS(&g_device_status, 0, kStatusBadPage);
-        return -1;
+// Where a token's row lies in the pools: its page is loaded when this is made, and looked at when the offset is asked for, so
+// that the load can be waited for behind other work.  offset(): elements from the k (which = 1) or v (2) pool's start, or -1
+// where the token is not stored: a negative position is padding; one behind its table row, or a page outside the pool, sets the
+// status word.
+struct Slot {
+    int64_t page, slot;
+    bool padding;
+    __device__ Slot(const RotArgs& a, int64_t tok, int64_t pos) {
+        padding = pos < 0;
+        page = -1;
+        slot = 0;
+        if (padding) return;
+        const int64_t seq = a.seq_ids ? (int64_t)a.seq_ids[tok] : tok;
+        int64_t at;
+        if (pos >> 32 | a.page_size >> 32) {
+            at = pos / a.page_size;
+        } else {                                 // (in 32 bits a tenth of the instructions in front of the load)
+            at = (uint32_t)pos / (uint32_t)a.page_size;
+        }
+        slot = pos - at * a.page_size;
+        if (seq >= 0 && seq < a.num_seqs && at < a.table_width) page = a.table[seq * a.table_stride + at];
     }
-    return page * a.r[which].db + (pos - at * a.page_size) * a.r[which].dl;
-}
+    __device__ int64_t offset(const RotArgs& a, int which) const {
+        if (padding) return -1;
+        if (page < 0 || page >= a.num_pages) {
+            atomicCAS(&g_device_status, 0, kStatusBadPage);
+            return -1;
+        }
+        return page * a.r[which].db + slot * a.r[which].dl;
+    }
+};
 
 using umma::f32x2;
 using umma::add2;
@@ -290,13 +307,12 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks) rotary_fwd_kernel(const 
     }
     if (!live) return;
     const int64_t pos = load_pos(a, b, l);
-    int64_t at = b * r.db + l * r.dl;
-    if (a.paged && which) {
-        at = slot_offset(a, tok, pos, which);
-        if (at < 0) return;
-    }
-    T* dst = static_cast<T*>(r.dst) + at + (first + slot) * r.dh + ln.ea;
+    const bool paged = a.paged && which;
+    const Slot where(a, tok, paged ? pos : -1);
     if (which < 2) stage_turns<N, LANES>(a, s_turn[warp], pos);
+    const int64_t at = paged ? where.offset(a, which) : b * r.db + l * r.dl;
+    if (paged && at < 0) return;
+    T* dst = static_cast<T*>(r.dst) + at + (first + slot) * r.dh + ln.ea;
     const bool norm = which < 2 && r.w;
     for (int h0 = 0; h0 < count; h0 += STEP) {
         uint4 u = nu, v = nv;
@@ -488,7 +504,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) rotary_fwd_any
     const int64_t pos = load_pos(a, b, l);
     T* y = static_cast<T*>(r.dst) + h * r.dh;
     if (a.paged && which) {
-        const int64_t at = slot_offset(a, tok, pos, which);
+        const int64_t at = Slot(a, tok, pos).offset(a, which);
         if (at < 0) return;
         y += at;
     } else {
