@@ -14,7 +14,7 @@
 // Measured (bf16, heads of 128, of the measured copy bandwidth): 32768 tokens x 64 heads turned in 167 us (0.98); 16384 tokens x
 // 40 heads normed and turned in 68 us (0.75: the norm's two waits for other lanes, and warps of 8 key heads that are short
 // beside their set-up), backward 100 us (0.77: registers, two blocks an SM); 9757 ragged tokens x 48 heads stored in pages in
-// 50 us (0.73); 64 tokens x 64 heads in 2.8 us, stored 3.8 us (the chain position -> table -> store behind the launch).
+// 50 us (0.73); 64 tokens x 64 heads in 2.8 us, stored 3.6 us (the chain position -> table -> store behind the launch).
 #include "attn.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
