@@ -5,7 +5,7 @@
 // in one pass over the cache with a running maximum m.  Every key and value is read once for up to 16 query heads, two
 // operations a byte and head: memory bounds it.  Measured (bf16, of the measured copy bandwidth): 64 sequences of 8192-8704
 // keys, 32 heads of 128, 1285-1320 us and one of 1,048,576 keys, 8 heads, 631 us (1.0); 32 sequences of 4000-8000 keys, 64
-// query heads over 8, 126-130 us (0.95); 48 ragged ones, 32 over 8 heads of 64 in fp16, 224 us (0.93); one of 700 keys 9.8 us
+// query heads over 8, 126-130 us (0.95); 48 ragged ones, 32 over 8 heads of 64 in fp16, 224 us (0.93); one of 700 keys 8.7 us
 // (a chain of launch, lengths, table, keys, join and join's launch).  What the kernels are built around:
 //
 // * Work.  The cache is cut into units of 64 or 128 keys of one key head; the units of all sequences, in a row, are dealt out in
@@ -705,29 +705,42 @@ template <typename T, int DP, int HP> __global__ void __launch_bounds__(kThreads
     __shared__ float2 s_ml[R];
     __shared__ __align__(16) float s_o[R][DP];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int w0 = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+    const int w0 = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, q = tid % Q, r0 = tid / Q;
+    const int run0 = w0 / a.abreast, runs = W / a.abreast;
+    // the run it begins in keeps it in slot 1, the others in slot 0
+    auto row = [&](int i) { return ((int64_t)(w0 + i * a.abreast) * 2 + (i == 0)) * HP + h; };
+    // the first rows are loaded before it is known whether this block has any (9.8 -> 8.7 us at one sequence of 700 keys)
+    constexpr int AHEAD = 4;
+    float2 ml[AHEAD];
+    float4 x[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+        if (run0 + r0 + j * R < runs) {
+            ml[j] = a.part_ml[row(r0 + j * R)];
+            x[j] = *reinterpret_cast<const float4*>(a.part + row(r0 + j * R) * DP + q * 4);
+        }
     const Open op = a.open[w0];
     if (op.b < 0) return;
     const int kvh = op.hg / a.passes, first = (op.hg - kvh * a.passes) * HP;
     if (first + h >= a.G) return;
-    const int n = op.runs, run0 = w0 / a.abreast, runs = W / a.abreast;
-    // the run it begins in keeps it in slot 1, the others in slot 0; a run may be empty
-    auto row = [&](int i) { return ((int64_t)(w0 + i * a.abreast) * 2 + (i == 0)) * HP + h; };
+    const int n = op.runs;
+    // a run may be empty where there are fewer units than runs
     const bool sparse = op.units < runs;
     auto empty = [&](int i) { return run_start(op.units, run0 + i, runs) == run_start(op.units, run0 + i + 1, runs); };
-    const int q = tid % Q, r0 = tid / Q;
     float m = -FLT_MAX, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = r0; i < n; i += R) {
-        if (sparse && empty(i)) continue;
-        const float2 ml = a.part_ml[row(i)];
-        const float4 x = *reinterpret_cast<const float4*>(a.part + row(i) * DP + q * 4);
+    auto add = [&](const float2& ml, const float4& x) {
         const float top = fmaxf(m, ml.x), f = exp2f(m - top), g = exp2f(ml.x - top);
         o.x = o.x * f + x.x * g; o.y = o.y * f + x.y * g; o.z = o.z * f + x.z * g; o.w = o.w * f + x.w * g;
         l = l * f + ml.y * g;
         m = top;
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+        if (r0 + j * R < n && !(sparse && empty(r0 + j * R))) add(ml[j], x[j]);
+#pragma unroll 4
+    for (int i = r0 + AHEAD * R; i < n; i += R)
+        if (!(sparse && empty(i))) add(a.part_ml[row(i)], *reinterpret_cast<const float4*>(a.part + row(i) * DP + q * 4));
     if (q == 0) s_ml[r0] = make_float2(m, l);
     *reinterpret_cast<float4*>(&s_o[r0][q * 4]) = o;
     __syncthreads();
