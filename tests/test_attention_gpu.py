@@ -93,6 +93,25 @@ def test_rotary_layouts(A, io, how):
     within(y, ref, R.norm_rotate_bound(ref, mag, dt), how)
 
 
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("H,D,rot", [(5, 64, 32), (33, 16, 16), (3, 20, 6), (2, 512, 512)])
+def test_rotary_in_place_through_the_c_abi(A, io, H, D, rot):
+    """The outputs are the inputs themselves: what the header allows and the wrapper does not use."""
+    import ctypes as C
+
+    from vortex_b200 import _lib
+    g, dt = gen(25), DT[io]
+    x, w = torch.randn(9, H, D, generator=g, device="cuda").to(dt), 1 + 0.1 * torch.randn(D, generator=g, device="cuda")
+    pos, fr = torch.arange(9, device="cuda") * 777, freqs(rot)
+    want = A.qk_norm_rotary(x, None, pos, fr, w, eps=EPS)
+    at = dict(B=1, L=9, Hq=H, D=D, rot=rot, scale=1.0, eps=EPS, io_dtype={"f32": 0, "bf16": 1}[io], positions=pos.data_ptr(), positions_i64=1,
+              pos_stride_l=1, inv_freq=fr.data_ptr(), inv_freq_f64=1, q_weight=w.data_ptr())
+    for n in ("q", "q_out"):
+        at.update({n: x.data_ptr(), n + "_stride_l": H * D, n + "_stride_h": D})
+    _lib.check(_lib.lib().vtx_qk_norm_rotary_fwd(C.byref(_lib.RotaryParams(**at)), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    assert torch.equal(x, want)
+
+
 def test_rotary_values_that_are_not_finite_stay_in_their_pair(A):
     x = torch.randn(1, 1, 64, generator=gen(4), device="cuda")
     x[0, 0, 3], x[0, 0, 40], x[0, 0, 63] = float("nan"), float("inf"), float("-inf")

@@ -298,7 +298,7 @@ class AttentionInferenceEngine:
     def decode(self, q, k, v):
         """One new token of every row of the cache, q [rows, Hq, D], k and v [rows, H, D], after ``cache.step``: stores its key
         and value and attends to the row's keys; rows without a sequence (or that ``step`` left out) give zeros.  Two calls,
-        three launches, no allocation but the outputs: can be captured and replayed."""
+        three launches, no allocation but the outputs and a workspace: can be captured and replayed."""
         from . import attn_ops
 
         c = self.cache
