@@ -850,3 +850,45 @@ def test_cache_copies_on_the_current_stream(A):
         got = [R.gather(cache.k[0], cache.block_table[r], cache.length(r)) for r in (b, c)]
     s.synchronize()
     assert torch.equal(got[0], x[6:]) and torch.equal(got[1], x[:6])
+
+
+@pytest.mark.parametrize("side", [0, 1])
+def test_rotary_second_gradients_raise_on_every_path(A, side):
+    """A gradient made with create_graph goes into what is differentiated again: an error wherever it depends on what is asked
+    for, also where another path reaches that; what it does not depend on is not touched by it."""
+    g = gen(40)
+    mk = lambda *s: torch.randn(*s, generator=g, device="cuda").requires_grad_()  # noqa: E731
+    x, other, w, c = mk(5, 2, 64), mk(5, 2, 64), mk(64), mk(5, 2, 64)
+    pos, fr = torch.arange(5, device="cuda"), freqs(64)
+    qk = (lambda w: A.qk_norm_rotary(x, other, pos, fr, w)) if side == 0 else (lambda w: A.qk_norm_rotary(other, x, pos, fr, None, w))
+
+    def once(f):
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            f()
+
+    y = qk(w)[side]
+    plain = torch.autograd.grad(y, [x, w], c, retain_graph=True)
+    gx, gw = torch.autograd.grad(y, [x, w], c, create_graph=True)
+    assert torch.equal(gx, plain[0]) and torch.equal(gw, plain[1])
+    for made in (gx, gw):
+        loss = y.sum() + made.pow(2).sum() + other.sum()
+        for leaf in (x, w, c):
+            once(lambda: torch.autograd.grad(loss, leaf, retain_graph=True))
+            once(lambda: torch.autograd.grad(made.sum(), leaf, retain_graph=True, allow_unused=True))
+            once(lambda: loss.backward(inputs=[leaf], retain_graph=True))
+        assert torch.equal(torch.autograd.grad(loss, other, retain_graph=True)[0], torch.ones_like(other))
+    # the other tensor's gradient is no function of this one, its own values or their weight
+    go = torch.autograd.grad(qk(w)[1 - side], other, c, create_graph=True)[0]
+    assert torch.autograd.grad(go.sum(), [x, w], retain_graph=True, allow_unused=True) == (None, None)
+    once(lambda: torch.autograd.grad(go.sum(), c, retain_graph=True))
+    # a rotation alone is linear: its gradient depends on the output's, not on the values
+    y = qk(None)[side]
+    gx = torch.autograd.grad(y, x, c, create_graph=True)[0]
+    once(lambda: torch.autograd.grad(gx.sum(), c, retain_graph=True))
+    assert torch.equal(torch.autograd.grad(y.sum() + gx.pow(2).sum(), x, retain_graph=True)[0], torch.autograd.grad(qk(None)[side].sum(), x)[0])
+    gx = torch.autograd.grad(y.pow(2).sum(), x, create_graph=True)[0]          # (here the output's gradient is one of the values)
+    once(lambda: torch.autograd.grad(y.sum() + gx.pow(2).sum(), x))
+    y = qk(w)[side]
+    gx = torch.autograd.grad(y.sum(), x, create_graph=True)[0]
+    once(lambda: (y.sum() + gx.pow(2).sum()).backward())
+    assert not torch.autograd.grad(qk(w)[side].sum(), x)[0].requires_grad

@@ -401,6 +401,25 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
         ctx->saved_data["scale"] = scale;
         return ko ? List{qo, *ko} : List{qo};
     }
+    // The gradients of a tensor and its weight, as functions of what they were formed from: the output's gradient dy, and behind
+    // a norm the tensor x and its weight w (without one the gradient is linear in dy).  There are no second derivatives, and a
+    // node with edges to all of these says so on whichever of them a second differentiation goes through; one without them
+    // would be passed over where only some inputs' gradients are asked for, and its part left out of the sum.
+    static void once(Tensor& gx, Tensor& gw, const Tensor& dy, const Tensor& x, const Tensor& w) {
+        List in{gx};
+        if (w.defined()) {
+            in.push_back(gw);
+            in.push_back(x);
+            in.push_back(w);
+        }
+        in.push_back(dy);
+        const int64_t n = (int64_t)in.size();
+        const auto node = std::make_shared<torch::autograd::DelayedError>(
+            "qk_norm_rotary can be differentiated once: its gradients must not have been used in what is differentiated again", n);
+        const List made = (*node)(std::move(in));
+        gx = made[0];
+        if (w.defined()) gw = made[1];
+    }
     static List backward(torch::autograd::AutogradContext* ctx, const List& grads) {
         const List saved = ctx->get_saved_variables();
         auto opt = [](const Tensor& t) { return t.defined() ? Opt(t) : Opt(); };
@@ -409,7 +428,6 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
         const Tensor &dq = grads[0], &q = norm ? saved[0] : dq;
         const Opt dk = grads.size() > 1 ? Opt(grads[1]) : Opt(), k = norm ? opt(saved[1]) : dk;
         List out(9);
-        bool again = at::GradMode::is_enabled();
         {
             const at::AutoGradMode off(false);
             auto [gq, gk, gqw, gkw] = qk_norm_rotary_bwd(dq, dk, q, k, saved[2], saved[3], qw, kw, ctx->saved_data["eps"].toDouble(),
@@ -419,13 +437,9 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
             if (gqw) out[4] = *gqw;
             if (gkw) out[5] = *gkw;
         }
-        bool needed = false;
-        for (const List* l : {&grads, &saved})
-            for (const Tensor& t : *l) needed = needed || (t.defined() && t.requires_grad());
-        if (again && needed) {                           // gradients of these gradients: an error where they are asked for
-            auto fn = std::make_shared<torch::autograd::DelayedError>("qk_norm_rotary can be differentiated once", 1);
-            for (const int i : {0, 1, 4, 5})
-                if (out[i].defined()) out[i] = (*fn)({out[i].detach().requires_grad_()})[0];
+        if (at::GradMode::is_enabled()) {                // (create_graph)
+            once(out[0], out[4], grads[0], saved[0], saved[4]);
+            if (dk) once(out[1], out[5], grads[1], saved[1], saved[5]);
         }
         return out;
     }
