@@ -892,3 +892,52 @@ def test_rotary_second_gradients_raise_on_every_path(A, side):
     gx = torch.autograd.grad(y.sum(), x, create_graph=True)[0]
     once(lambda: (y.sum() + gx.pow(2).sum()).backward())
     assert not torch.autograd.grad(qk(w)[side].sum(), x)[0].requires_grad
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("D", [64, 128, 40])
+def test_decode_attention_of_no_key_at_all(A, io, page, D):
+    """A sequence whose counted keys all lie in pages that the table does not give: zeros and -inf, as for one of length 0,
+    finished by one block (short) or joined from several (long).  Keys that are there and whose scores are all -inf: the formula's
+    0 / 0.  Some of each: the others' softmax."""
+    from vortex_b200 import ops
+    ops.device_status()
+    g, dt, H = gen(43), DT[io], 2
+    kp, vp = pools(g, 300, page, 1, D, dt)
+    width = 1200 // page
+    order = torch.randperm(300, generator=g, device="cuda").to(torch.int32)
+    q = torch.randn(4, H, D, generator=g, device="cuda").to(dt)
+    for n, window in ((3, 0), (1200 // page * page, 0), (1000, 900)):
+        table = torch.stack([order[:width], torch.full((width,), -1, device="cuda", dtype=torch.int32), order[-width:].flip(0),
+                             torch.full((width,), 300, device="cuda", dtype=torch.int32)])
+        if window:
+            table[1, :(n - window) // page] = 7                  # pages before the window are there and do not count
+        lens = torch.tensor([n, n, 0, n], dtype=torch.int32, device="cuda")
+        out, lse = A.paged_decode_attention(q, kp, vp, table, lens, window=window, return_lse=True)
+        with pytest.raises(RuntimeError, match="block table"):
+            ops.device_status()
+        ref, _, bound = R.attend(q[:1], kp, vp, table[:1], [n], D ** -0.5, window)
+        within(out[:1], ref, bound + R.rounding(ref.abs() + bound, dt), "first")
+        assert not bool(out[1:].any()) and bool(lse[1:].isneginf().all()) and bool(lse[0].isfinite().all())
+    # scores of -inf: a key of -inf in a value where every query is 1, the others 0
+    q[..., 0] = 1.0
+    table[1], table[2], table[3] = order[:width], order[:width], order[:width]
+    for n in (3, 1200 // page * page):
+        kk = kp.clone()
+        kk[..., 0] = float("-inf")
+        lens = torch.tensor([n, n, n, n], dtype=torch.int32, device="cuda")
+        table[3] = -1
+        table[3, 0] = order[0]
+        out, lse = A.paged_decode_attention(q, kk, vp, table, lens, return_lse=True)
+        if n > page:
+            with pytest.raises(RuntimeError, match="block table"):
+                ops.device_status()
+        assert bool(out.isnan().all()) and bool(lse.isneginf().all())
+        kk = kp.clone()
+        kk[order[0].long(), 0, :, 0] = float("-inf")            # one key, the first of each, beside finite ones
+        out, lse = A.paged_decode_attention(q[:1], kk, vp, table[:1], lens[:1], return_lse=True)
+        ref, _, bound = R.attend(q[:1], kp, vp, table[:1], [n], D ** -0.5, n - 1)
+        within(out, ref, bound + R.rounding(ref.abs() + bound, dt), "rest")
+        assert bool(lse.isfinite().all())
+    ops.device_status()
