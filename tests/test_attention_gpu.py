@@ -941,3 +941,23 @@ def test_decode_attention_of_no_key_at_all(A, io, page, D):
         within(out, ref, bound + R.rounding(ref.abs() + bound, dt), "rest")
         assert bool(lse.isfinite().all())
     ops.device_status()
+
+
+def test_rotary_refuses_forward_mode_derivatives(A):
+    """A tangent would be lost: the call says so, with and without gradients recorded; duals nearby do not matter."""
+    import torch.autograd.forward_ad as fwd
+    g = gen(41)
+    x, w = torch.randn(3, 2, 64, generator=g, device="cuda"), torch.ones(64, device="cuda")
+    pos, fr = torch.arange(3, device="cuda"), freqs(64)
+    want = A.qk_norm_rotary(x, x, pos, fr, w, w)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        dx, dw, df = dual(x), dual(w), dual(fr)
+        for args in ((dx, x, pos, fr, w, w), (x, dx, pos, fr, w, w), (x, x, pos, fr, dw, w), (x, x, pos, fr, w, dw), (x, x, pos, df),
+                     (dx, None, pos, fr)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                A.qk_norm_rotary(*args)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                A.qk_norm_rotary(*args)
+        got = A.qk_norm_rotary(x, x, pos, fr, w, w)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -64,7 +64,8 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, e
     ``interleaved``, else (i, i + rot / 2); rotated values are multiplied by ``scale``, the others kept.  ``positions`` are
     int32 or int64, [T], [B, L] or [L] for every batch element; ``inv_freq`` float64 (or float32) on the device, see
     ``rotary_inv_freq``.  Angles are formed in 64 bits, the rest in fp32, rounded once.  Differentiable in q, k and the
-    weights (once); the weights' gradients are summed in a fixed order.  D <= 512."""
+    weights, once and in reverse mode (a second differentiation raises, as forward mode does); the weights' gradients are
+    summed in a fixed order.  D <= 512."""
     qo, ko = ops.qk_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, eps=eps, interleaved=interleaved, scale=scale)
     return qo if k is None else (qo, ko)
 

@@ -447,6 +447,9 @@ struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
 
 std::tuple<Tensor, Opt> qk_norm_rotary_grad(const Tensor& q, const Opt& k, const Tensor& positions, const Tensor& inv_freq, const Opt& qw, const Opt& kw,
                                             double eps, bool interleaved, double scale) {
+    auto dual = [](const Opt& t) { return t && t->_fw_grad(/*level=*/0).defined(); };
+    if (dual(q) || dual(k) || dual(inv_freq) || dual(qw) || dual(kw))            // (the kernel would drop the tangent)
+        raise(PyExc_NotImplementedError, "qk_norm_rotary has no forward-mode derivative");
     auto wants = [](const Opt& t) { return t && t->requires_grad(); };
     if (!at::GradMode::is_enabled() || !(q.requires_grad() || wants(k) || wants(qw) || wants(kw)))
         return qk_norm_rotary(q, k, positions, inv_freq, qw, kw, eps, interleaved, scale);
