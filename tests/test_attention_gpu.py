@@ -961,3 +961,37 @@ def test_rotary_refuses_forward_mode_derivatives(A):
                 A.qk_norm_rotary(*args)
         got = A.qk_norm_rotary(x, x, pos, fr, w, w)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_written_pools_say_so_to_autograd(A):
+    """A call that writes pools raises their version (views of one tensor share it): a product that saved one before and is
+    differentiated after raises instead of using what lies there by then.  Pools made in inference mode have no version."""
+    g = gen(42)
+    kv = torch.randn(4, 16, 2, 2, 64, generator=g, device="cuda")
+    kp, vp = kv[:, :, 0], kv[:, :, 1]
+    x = torch.randn(2, 2, 64, generator=g, device="cuda")
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([3, 4], dtype=torch.int32, device="cuda")
+    calls = {"append": lambda k, v: A.rotary_append(x, x, x, pos, k, v, table), "copy": lambda k, v: A.copy_pages([k, v], [0], [2])}
+    a = torch.ones(4, 16, 2, 64, device="cuda", requires_grad=True)
+    for name, call in calls.items():
+        for k, v in ((kp, vp), (torch.zeros(4, 16, 2, 64, device="cuda"), torch.zeros(4, 16, 2, 64, device="cuda"))):
+            if name == "copy":
+                k, v = k.contiguous().clone(), v.contiguous().clone()
+            before, saved = (k._version, v._version), ((a * k).sum(), (a * v).sum())
+            call(k, v)
+            assert k._version > before[0] and v._version > before[1], name
+            for s in saved:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    s.backward()
+        with torch.inference_mode():
+            k, v = (torch.zeros(4, 16, 2, 64, device="cuda") for _ in range(2))
+            call(k, v)
+        call(k, v)
+    q = torch.randn(2, 2, 64, generator=g, device="cuda")
+    lens = torch.tensor([4, 5], dtype=torch.int32, device="cuda")
+    kp, vp = kp.contiguous(), vp.contiguous()
+    before = kp._version, vp._version, q._version
+    A.paged_decode_attention(q, kp, vp, table, lens)
+    A.qk_norm_rotary(q, None, pos, freqs(64))
+    assert (kp._version, vp._version, q._version) == before

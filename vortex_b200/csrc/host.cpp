@@ -73,6 +73,11 @@ Opt param(const Opt& t, const Tensor& like) { return t ? Opt(param(*t, like)) : 
 const void* ptr(const Tensor& t) { return t.const_data_ptr(); }
 const void* ptr(const Opt& t) { return t ? t->const_data_ptr() : nullptr; }
 void* out(const Tensor& t) { return t.mutable_data_ptr(); }
+// A tensor that the caller owns is written: autograd then sees that what it may have saved of it is gone.  (Tensors made in
+// inference mode carry no version.)
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 int64_t code_or_0(const Opt& t) { return t ? code(*t) : 0; }
 // (straight to the CUDA allocator: at::empty's way through the dispatcher costs another half microsecond)
 Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType dtype) {
@@ -506,6 +511,7 @@ Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const
     }
     const c10::cuda::CUDAGuard on(q.t.device());
     check(p_rotary_append(&p, stream_of(q.t)));
+    written(k_pages); written(v_pages);
     return qo;
 }
 
@@ -569,6 +575,7 @@ void copy_pages(const std::vector<Tensor>& pools, const std::vector<int64_t>& sr
     p.page_bytes = page * es; p.page_stride_bytes = n > 1 ? first.stride(0) * es : page * es;
     const c10::cuda::CUDAGuard on(first.device());
     check(p_copy_pages(&p, stream_of(first)));
+    if (p.pairs) for (const Tensor& t : pools) written(t);
 }
 
 }  // namespace
