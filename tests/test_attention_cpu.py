@@ -254,3 +254,63 @@ def test_cache_refusals_change_nothing(host_copies):
         c.free(b)
     with pytest.raises(ValueError):
         cache(page_size=0)
+
+
+@pytest.mark.parametrize("call", ["extend", "extend none", "step", "step some", "fork", "fork shared", "free", "compact"])
+def test_cache_calls_that_fail_on_the_way_change_nothing(host_copies, monkeypatch, call):
+    """Each upload and page copy of a call fails in turn: bookkeeping, table, positions and lengths are as before it, and the
+    same call afterwards does what it would have done."""
+    from vortex_b200 import attn_ops
+    made = {"extend": lambda c: c.extend([0, 2], [6, 3]), "extend none": lambda c: c.extend([0], [0]), "step": lambda c: c.step(),
+            "step some": lambda c: c.step([2]), "fork": lambda c: c.fork(0), "fork shared": lambda c: c.fork(2), "free": lambda c: c.free(0),
+            "compact": lambda c: c.compact()}[call]
+
+    def start():
+        c = cache()
+        for _ in range(3):
+            c.open()
+        pos, seq = c.extend([0, 1, 2], [7, 9, 8])
+        store(c, pos, seq, [float(i) for i in range(24)])
+        c.step([1])
+        c.free(1)
+        c.step([0])
+        store(c, torch.tensor([7]), torch.tensor([0]), [30.0])
+        return c
+
+    def state(c):
+        rows = [r for r, p in enumerate(c._pages) if p is not None]
+        return (rows, [c.pages(r) for r in rows], [c.length(r) for r in rows], [held(c, r) for r in rows], sorted(c._unused), list(c._users),
+                c.block_table.tolist(), c._table.tolist(), c.positions.tolist(), c.lengths.tolist())
+
+    left = [None]
+
+    def failing(f):
+        def g(*a, **kw):
+            if left[0] is not None:
+                left[0] -= 1
+                if left[0] < 0:
+                    left[0] = None
+                    raise RuntimeError("planted")
+            return f(*a, **kw)
+        return g
+
+    for name in ("copy_", "to"):
+        monkeypatch.setattr(torch.Tensor, name, failing(getattr(torch.Tensor, name)))
+    monkeypatch.setattr(attn_ops, "copy_pages", failing(attn_ops.copy_pages))
+    good = start()
+    made(good)
+    for n in range(10):
+        c = start()
+        before = state(c)
+        left[0] = n
+        try:
+            made(c)
+        except RuntimeError as e:
+            assert str(e) == "planted"
+            assert state(c) == before
+            made(c)
+            assert state(c) == state(good)
+        else:
+            left[0] = None
+            break
+    assert 0 < n < 10

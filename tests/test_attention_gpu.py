@@ -995,3 +995,28 @@ def test_written_pools_say_so_to_autograd(A):
     A.paged_decode_attention(q, kp, vp, table, lens)
     A.qk_norm_rotary(q, None, pos, freqs(64))
     assert (kp._version, vp._version, q._version) == before
+
+
+def test_cache_refuses_to_change_under_capture(A):
+    """Its uploads would not be part of the graph: refused before anything is changed, the capture goes on and replays."""
+    from vortex_b200 import AttentionInferenceEngine, PagedKVCache
+    cache = PagedKVCache(1, 8, 4, 1, 64, max_sequences=3, max_length=16)
+    layer = AttentionInferenceEngine(cache, 0, A.rotary_inv_freq(64)[0])
+    a, b = cache.open(), cache.open()
+    cache.extend([a, b], [4, 3])
+    cache.step([a])
+    x = torch.randn(3, 1, 64, generator=gen(44), device="cuda").bfloat16()
+    eager = layer.decode(x, x, x)
+    torch.cuda.synchronize()
+    now = lambda: ([cache.pages(r) for r in (a, b)], [cache.length(r) for r in (a, b)], cache.unused_pages)  # noqa: E731
+    before, device = now(), (cache.block_table.clone(), cache.positions.clone(), cache.lengths.clone())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for f in (cache.step, lambda: cache.step([b]), lambda: cache.extend([a], [2]), lambda: cache.fork(b), lambda: cache.free(a), cache.compact):
+            with pytest.raises(RuntimeError, match="capture"):
+                f()
+            assert now() == before
+        out = layer.decode(x, x, x)
+    assert now() == before and all(torch.equal(p, q) for p, q in zip(device, (cache.block_table, cache.positions, cache.lengths)))
+    graph.replay()
+    assert torch.equal(out, eager)

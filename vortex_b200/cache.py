@@ -9,6 +9,7 @@ dictionaries, keyed by layer index:
 Prefill writes the FIR caches in the activation dtype; every decode step returns them in fp32
 (``vortex/model/engine.py:427-449``).
 """
+import contextlib
 import heapq
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
@@ -75,8 +76,9 @@ class PagedKVCache:
     addresses: a captured decode step follows what ``step`` puts there before each replay.
 
     ``open`` / ``extend`` / ``step`` / ``free`` change the bookkeeping on the host and upload what changed on the current
-    stream; ``fork`` and ``compact`` copy pages as well (``attn_ops.copy_pages``).  None of them may run under stream
-    capture.  A call that raises has changed nothing.  Not thread-safe."""
+    stream; ``fork`` and ``compact`` copy pages as well (``attn_ops.copy_pages``).  Under stream capture all but ``open`` are
+    refused: their uploads would not be part of the graph.  A call that raises has changed nothing (bookkeeping follows the
+    uploads; one that fails after another is done takes that back).  Not thread-safe."""
 
     def __init__(self, layers, num_pages, page_size, num_heads, head_dim, *, max_sequences, max_length, device="cuda",
                  dtype=torch.bfloat16):
@@ -114,17 +116,50 @@ class PagedKVCache:
         if not 0 <= row < len(self._pages) or self._pages[row] is None:
             raise ValueError(f"row {row} holds no sequence")
 
-    def _take(self) -> int:
-        page = heapq.heappop(self._unused)
-        self._users[page] = 1
-        return page
+    def _take(self, count: int) -> list[int]:
+        """The lowest unused pages, out of the heap but not yet anyone's."""
+        if count > len(self._unused):
+            raise RuntimeError(f"{count} page{'s' if count > 1 else ''} needed, {len(self._unused)} unused")
+        return [heapq.heappop(self._unused) for _ in range(count)]
+
+    def _put_back(self, pages) -> None:
+        for page in pages:
+            heapq.heappush(self._unused, page)
+
+    def _not_captured(self) -> None:
+        if self.block_table.is_cuda:
+            with torch.cuda.device(self.block_table.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a paged cache cannot be changed under stream capture")
 
     def _upload(self, rows: Sequence[int]) -> None:
         """The rows' part of the table, in one copy.  (From pageable memory, which CUDA has read when the call returns: the
-        host's copy may change afterwards, and nothing waits for the stream.)"""
+        host's copy may change afterwards.  Whether the driver waits for the stream meanwhile is up to it.)"""
         if rows:
             lo, hi = min(rows), max(rows) + 1
             self.block_table[lo:hi].copy_(self._table[lo:hi], non_blocking=True)
+
+    def _change_table(self, entries, then=None):
+        """Table entries {row: (first entry, pages)} on the host and the device, then whatever else the call has to upload;
+        returns what that returns.  If any of it raises, the table is as it was."""
+        rows = [row for row, (_, pages) in entries.items() if len(pages)]
+        before, done = [], False
+        try:
+            for row in rows:
+                first, pages = entries[row]
+                part = self._table[row, first:first + len(pages)]
+                before.append((part, part.clone()))
+                part[:] = torch.tensor(pages, dtype=torch.int32)
+            self._upload(rows)
+            done = True
+            return then() if then else None
+        except BaseException:
+            for part, was in before:
+                part[:] = was
+            if done:
+                with contextlib.suppress(Exception):
+                    self._upload(rows)
+            raise
 
     # -- sequences
     def open(self) -> int:
@@ -135,28 +170,33 @@ class PagedKVCache:
                 return row
         raise RuntimeError(f"all {len(self._pages)} rows hold sequences")
 
-    def _grow(self, rows, counts) -> None:
-        """Room for counts[i] more tokens of rows[i]: bookkeeping and table."""
+    def _grow(self, rows, counts, upload):
+        """Room for counts[i] more tokens of rows[i]; returns what ``upload`` returns, which is called when the table is there."""
+        self._not_captured()
         if len(set(rows)) != len(rows):
             raise ValueError("a row occurs twice")
-        need = 0
+        need = []
         for row, n in zip(rows, counts):
             self._check(row)
             if n < 0 or self._length[row] + n > self.max_length:
                 raise ValueError(f"row {row}: {self._length[row]} + {n} tokens of at most {self.max_length}")
-            need += -(-(self._length[row] + n) // self.page_size) - len(self._pages[row])
-        if need > len(self._unused):
-            raise RuntimeError(f"{need} pages needed, {len(self._unused)} unused")
-        changed = []
+            need.append(-(-(self._length[row] + n) // self.page_size) - len(self._pages[row]))
+        taken = self._take(sum(need))
+        new, at = {}, 0
+        for row, n in zip(rows, need):
+            new[row] = (len(self._pages[row]), taken[at:at + n])
+            at += n
+        try:
+            made = self._change_table(new, upload)
+        except BaseException:
+            self._put_back(taken)
+            raise
         for row, n in zip(rows, counts):
             self._length[row] += n
-            pages = self._pages[row]
-            while len(pages) * self.page_size < self._length[row]:
-                self._table[row, len(pages)] = page = self._take()
-                pages.append(page)
-                if not changed or changed[-1] != row:
-                    changed.append(row)
-        self._upload(changed)
+            self._pages[row] += new[row][1]
+        for page in taken:
+            self._users[page] = 1
+        return made
 
     def extend(self, rows: Sequence[int], counts: Sequence[int]):
         """Room for ``counts[i]`` new tokens of sequence ``rows[i]``; returns their positions and rows (int32, on the device),
@@ -165,69 +205,76 @@ class PagedKVCache:
         if len(rows) != len(counts):
             raise ValueError("one count for every row")
         first = [self.length(row) for row in rows]
-        self._grow(rows, counts)
-        both = torch.empty(2, sum(counts), dtype=torch.int32)
-        at = 0
-        for row, start, n in zip(rows, first, counts):
-            both[0, at:at + n] = torch.arange(start, start + n, dtype=torch.int32)
-            both[1, at:at + n] = row
-            at += n
-        both = both.to(self.block_table.device, non_blocking=True)
+
+        def upload():
+            both = torch.empty(2, sum(counts), dtype=torch.int32)
+            at = 0
+            for row, start, n in zip(rows, first, counts):
+                both[0, at:at + n] = torch.arange(start, start + n, dtype=torch.int32)
+                both[1, at:at + n] = row
+                at += n
+            return both.to(self.block_table.device, non_blocking=True)
+
+        both = self._grow(rows, counts, upload)
         return both[0], both[1]
 
     def step(self, rows: Optional[Sequence[int]] = None) -> None:
         """Room for one new token of each of ``rows`` (None: every open sequence); ``positions`` and ``lengths`` say so to
         the decode step that follows."""
         rows = [r for r, p in enumerate(self._pages) if p is not None] if rows is None else list(rows)
-        self._grow(rows, [1] * len(rows))
-        both = torch.zeros(2, len(self._pages), dtype=torch.int32)
-        both[0] = -1
-        for row in rows:
-            both[0, row], both[1, row] = self._length[row] - 1, self._length[row]
-        self._step.copy_(both, non_blocking=True)
+
+        def upload():
+            positions, lengths = [-1] * len(self._pages), [0] * len(self._pages)
+            for row in rows:
+                positions[row], lengths[row] = self._length[row], self._length[row] + 1
+            self._step.copy_(torch.tensor([positions, lengths], dtype=torch.int32), non_blocking=True)
+
+        self._grow(rows, [1] * len(rows), upload)
 
     def fork(self, row: int) -> int:
         """A sequence that begins as a copy of ``row``: full pages are shared, an open last page is copied in every pool.
-        Returns its row."""
+        Returns its row.  What it holds is what the stream has stored by then: tokens that ``extend`` or ``step`` made room
+        for are stored first."""
+        self._not_captured()
         self._check(row)
-        open_page = self._length[row] % self.page_size != 0
-        if open_page and not self._unused:
-            raise RuntimeError("1 page needed, 0 unused")
-        child = self.open()
         pages = list(self._pages[row])
-        if open_page:
-            from . import attn_ops
+        own = self._take(1) if self._length[row] % self.page_size else []
+        child = None
+        try:
+            child = self.open()
+            if own:
+                from . import attn_ops
 
-            page = self._unused[0]
-            try:
-                attn_ops.copy_pages(self.k + self.v, [pages[-1]], [page])
-            except Exception:
+                attn_ops.copy_pages(self.k + self.v, pages[-1:], own)
+                pages[-1:] = own
+            self._change_table({child: (0, pages)})
+        except BaseException:
+            self._put_back(own)
+            if child is not None:
                 self._pages[child] = None
-                raise
-            pages[-1] = self._take()
-        for page in pages[:-1] if open_page else pages:
+            raise
+        for page in pages:
             self._users[page] += 1
         self._pages[child], self._length[child] = pages, self._length[row]
-        self._table[child, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
-        self._upload([child])
         return child
 
     def free(self, row: int) -> None:
         """Ends a sequence; pages that no other sequence holds are unused again."""
+        self._not_captured()
         self._check(row)
+        self._change_table({row: (0, [-1] * len(self._pages[row]))})
         for page in self._pages[row]:
             self._users[page] -= 1
             if self._users[page] == 0:
                 heapq.heappush(self._unused, page)
         self._pages[row], self._length[row] = None, 0
-        self._table[row] = -1
-        self._upload([row])
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest numbers and returns how many there are: what lies behind them in the pools
         is free to be given back or reused."""
         from . import attn_ops
 
+        self._not_captured()
         used = self.num_pages - len(self._unused)
         src = [p for p in range(used, self.num_pages) if self._users[p]]
         dst = sorted(p for p in self._unused if p < used)
@@ -235,14 +282,11 @@ class PagedKVCache:
             return used
         attn_ops.copy_pages(self.k + self.v, src, dst)
         to = dict(zip(src, dst))
-        changed = []
-        for row, pages in enumerate(self._pages):
-            if pages and any(p in to for p in pages):
-                self._pages[row] = pages = [to.get(p, p) for p in pages]
-                self._table[row, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
-                changed.append(row)
+        moved = {row: [to.get(p, p) for p in pages] for row, pages in enumerate(self._pages) if pages and any(p in to for p in pages)}
+        self._change_table({row: (0, pages) for row, pages in moved.items()})
+        for row, pages in moved.items():
+            self._pages[row] = pages
         for a, b in to.items():
             self._users[b], self._users[a] = self._users[a], 0
         self._unused = list(range(used, self.num_pages))
-        self._upload(changed)
         return used
