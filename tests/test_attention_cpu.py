@@ -314,3 +314,19 @@ def test_cache_calls_that_fail_on_the_way_change_nothing(host_copies, monkeypatc
             left[0] = None
             break
     assert 0 < n < 10
+
+
+def test_cache_step_without_a_sequence_that_ended(host_copies):
+    """free between step and the decode step: the row is in the step no more, nor one that is opened in its place."""
+    c = cache()
+    a, b = c.open(), c.open()
+    c.extend([a, b], [5, 3])
+    c.step()
+    assert c.positions.tolist() == [5, 3, -1, -1, -1] and c.lengths.tolist() == [6, 4, 0, 0, 0]
+    c.free(a)
+    assert c.positions.tolist() == [-1, 3, -1, -1, -1] and c.lengths.tolist() == [0, 4, 0, 0, 0]
+    assert c.open() == a
+    c.extend([a], [2])
+    assert c.positions.tolist() == [-1, 3, -1, -1, -1] and c.lengths.tolist() == [0, 4, 0, 0, 0]
+    c.step()
+    assert c.positions.tolist() == [2, 4, -1, -1, -1] and c.lengths.tolist() == [3, 5, 0, 0, 0]

@@ -1020,3 +1020,22 @@ def test_cache_refuses_to_change_under_capture(A):
     assert now() == before and all(torch.equal(p, q) for p, q in zip(device, (cache.block_table, cache.positions, cache.lengths)))
     graph.replay()
     assert torch.equal(out, eager)
+
+
+def test_a_sequence_that_ends_between_step_and_decode(A):
+    """Its row stores nothing, gives zeros and reports nothing; the others are as without it."""
+    from vortex_b200 import AttentionInferenceEngine, PagedKVCache, ops
+    ops.device_status()
+    g = gen(45)
+    cache = PagedKVCache(1, 8, 4, 1, 64, max_sequences=3, max_length=16)
+    layer = AttentionInferenceEngine(cache, 0, A.rotary_inv_freq(64)[0])
+    a, b = cache.open(), cache.open()
+    pos, seq = cache.extend([a, b], [6, 5])
+    x, y = (torch.randn(n, 1, 64, generator=g, device="cuda").bfloat16() for n in (11, 3))
+    layer.prefill(x, x, x, pos, seq)
+    cache.step()
+    want = layer.decode(y, y, y)
+    cache.free(a)
+    got = layer.decode(y, y, y)                 # the same step again, without the first row
+    ops.device_status()
+    assert not bool(got[a].any()) and torch.equal(got[b], want[b])

@@ -93,6 +93,7 @@ class PagedKVCache:
         self._step = torch.zeros(2, max_sequences, device=device, dtype=torch.int32)
         self._step[0] = -1
         self.positions, self.lengths = self._step[0], self._step[1]
+        self._at_work = ([-1] * max_sequences, [0] * max_sequences)                  # the host's copy of these two
         self._table = torch.full((max_sequences, width), -1, dtype=torch.int32)      # the host's copy
         self._pages: list[Optional[list[int]]] = [None] * max_sequences              # of each open row
         self._length = [0] * max_sequences
@@ -138,6 +139,9 @@ class PagedKVCache:
         if rows:
             lo, hi = min(rows), max(rows) + 1
             self.block_table[lo:hi].copy_(self._table[lo:hi], non_blocking=True)
+
+    def _upload_step(self, at_work) -> None:
+        self._step.copy_(torch.tensor(at_work, dtype=torch.int32), non_blocking=True)
 
     def _change_table(self, entries, then=None):
         """Table entries {row: (first entry, pages)} on the host and the device, then whatever else the call has to upload;
@@ -227,9 +231,10 @@ class PagedKVCache:
             positions, lengths = [-1] * len(self._pages), [0] * len(self._pages)
             for row in rows:
                 positions[row], lengths[row] = self._length[row], self._length[row] + 1
-            self._step.copy_(torch.tensor([positions, lengths], dtype=torch.int32), non_blocking=True)
+            self._upload_step((positions, lengths))
+            return positions, lengths
 
-        self._grow(rows, [1] * len(rows), upload)
+        self._at_work = self._grow(rows, [1] * len(rows), upload)
 
     def fork(self, row: int) -> int:
         """A sequence that begins as a copy of ``row``: full pages are shared, an open last page is copied in every pool.
@@ -259,10 +264,15 @@ class PagedKVCache:
         return child
 
     def free(self, row: int) -> None:
-        """Ends a sequence; pages that no other sequence holds are unused again."""
+        """Ends a sequence; pages that no other sequence holds are unused again, and the step at work, if the row is in it, goes
+        on without."""
         self._not_captured()
         self._check(row)
-        self._change_table({row: (0, [-1] * len(self._pages[row]))})
+        positions, lengths = map(list, self._at_work)
+        in_step = lengths[row] > 0
+        positions[row], lengths[row] = -1, 0
+        self._change_table({row: (0, [-1] * len(self._pages[row]))}, (lambda: self._upload_step((positions, lengths))) if in_step else None)
+        self._at_work = positions, lengths
         for page in self._pages[row]:
             self._users[page] -= 1
             if self._users[page] == 0:
