@@ -330,3 +330,18 @@ def test_cache_step_without_a_sequence_that_ended(host_copies):
     assert c.positions.tolist() == [-1, 3, -1, -1, -1] and c.lengths.tolist() == [0, 4, 0, 0, 0]
     c.step()
     assert c.positions.tolist() == [2, 4, -1, -1, -1] and c.lengths.tolist() == [3, 5, 0, 0, 0]
+
+
+def test_cache_under_another_default_device(host_copies):
+    """The host's side stays on the host."""
+    with torch.device("meta"):
+        c = cache()
+        a = c.open()
+        pos, seq = c.extend([a], [6])
+        c.step()
+        b = c.fork(a)
+        c.free(a)
+        assert c.compact() == 2
+    assert all(t.device.type == "cpu" for t in (c._table, c.block_table, c.positions, pos, seq, *c.k))
+    assert pos.tolist() == list(range(6)) and seq.tolist() == [a] * 6 and c.block_table[b, :2].tolist() == c.pages(b)
+    assert c.positions[a] == -1 and c.length(b) == 7

@@ -94,7 +94,7 @@ class PagedKVCache:
         self._step[0] = -1
         self.positions, self.lengths = self._step[0], self._step[1]
         self._at_work = ([-1] * max_sequences, [0] * max_sequences)                  # the host's copy of these two
-        self._table = torch.full((max_sequences, width), -1, dtype=torch.int32)      # the host's copy
+        self._table = torch.full((max_sequences, width), -1, device="cpu", dtype=torch.int32)      # the host's copy
         self._pages: list[Optional[list[int]]] = [None] * max_sequences              # of each open row
         self._length = [0] * max_sequences
         self._users = [0] * num_pages                                                # rows that hold a page
@@ -141,7 +141,7 @@ class PagedKVCache:
             self.block_table[lo:hi].copy_(self._table[lo:hi], non_blocking=True)
 
     def _upload_step(self, at_work) -> None:
-        self._step.copy_(torch.tensor(at_work, dtype=torch.int32), non_blocking=True)
+        self._step.copy_(torch.tensor(at_work, device="cpu", dtype=torch.int32), non_blocking=True)
 
     def _change_table(self, entries, then=None):
         """Table entries {row: (first entry, pages)} on the host and the device, then whatever else the call has to upload;
@@ -153,7 +153,7 @@ class PagedKVCache:
                 first, pages = entries[row]
                 part = self._table[row, first:first + len(pages)]
                 before.append((part, part.clone()))
-                part[:] = torch.tensor(pages, dtype=torch.int32)
+                part[:] = torch.tensor(pages, device="cpu", dtype=torch.int32)
             self._upload(rows)
             done = True
             return then() if then else None
@@ -211,10 +211,10 @@ class PagedKVCache:
         first = [self.length(row) for row in rows]
 
         def upload():
-            both = torch.empty(2, sum(counts), dtype=torch.int32)
+            both = torch.empty(2, sum(counts), device="cpu", dtype=torch.int32)
             at = 0
             for row, start, n in zip(rows, first, counts):
-                both[0, at:at + n] = torch.arange(start, start + n, dtype=torch.int32)
+                both[0, at:at + n] = torch.arange(start, start + n, device="cpu", dtype=torch.int32)
                 both[1, at:at + n] = row
                 at += n
             return both.to(self.block_table.device, non_blocking=True)
