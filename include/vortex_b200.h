@@ -549,7 +549,9 @@ int vtx_rotary_append(const vtx_rotary_append_params* p, void* stream);
  * that lie behind its width, are left out and set the device status word.
  * fp32 accumulation; probabilities enter the second product as head and remainder of the I/O dtype.  D <= 256.
  * scratch: vtx_paged_decode_scratch_bytes(p) bytes, 16-byte aligned, its contents of no meaning before and after the call
- * (two calls that may overlap need two).  The reference calls flash_attn_with_kvcache (vortex/ops/attn_interface.py:1488). */
+ * (two calls that may overlap need two).  The bytes grow with the batch, the heads and the keys that the table or cache has room
+ * for, and depend on the pointers' and strides' alignment, which selects the kernel: ask with the parameters of the call.  They
+ * never exceed VTX_PAGED_DECODE_SCRATCH_MAX, which serves every call.  The reference calls flash_attn_with_kvcache (vortex/ops/attn_interface.py:1488). */
 typedef struct vtx_paged_decode_params {
     const void* q;  int64_t q_stride_b, q_stride_h;
     const void* k_pages; int64_t k_stride_page, k_stride_slot, k_stride_head;
@@ -565,6 +567,7 @@ typedef struct vtx_paged_decode_params {
     int64_t num_pages, page_size;
     int64_t io_dtype;
 } vtx_paged_decode_params;
+#define VTX_PAGED_DECODE_SCRATCH_MAX (5 << 20)
 int64_t vtx_paged_decode_scratch_bytes(const vtx_paged_decode_params* p);
 int vtx_paged_decode_attention(const vtx_paged_decode_params* p, void* stream);
 

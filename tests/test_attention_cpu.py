@@ -345,3 +345,22 @@ def test_cache_under_another_default_device(host_copies):
     assert all(t.device.type == "cpu" for t in (c._table, c.block_table, c.positions, pos, seq, *c.k))
     assert pos.tolist() == list(range(6)) and seq.tolist() == [a] * 6 and c.block_table[b, :2].tolist() == c.pages(b)
     assert c.positions[a] == -1 and c.length(b) == 7
+
+
+def test_decode_attention_scratch_maximum():
+    """More for a larger batch at one table width, and for other alignments; never beyond the header's maximum, nor its document."""
+    import itertools
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "include", "vortex_b200.h")) as f:
+        n, shift = map(int, re.search(r"VTX_PAGED_DECODE_SCRATCH_MAX \((\d+) << (\d+)\)", f.read()).groups())
+    with open(os.path.join(root, "INTEGRATION.md")) as f:
+        assert "does not grow" not in f.read()
+    f = _lib.lib().vtx_paged_decode_scratch_bytes
+    need = lambda **kw: f(C.byref(decode(**kw)))  # noqa: E731
+    assert need(B=1) < need(B=16) < need(B=256)
+    assert need(B=64, q=16) != need(B=64, q=18)
+    for io, D, (Hq, Hk), B, width, q, table in itertools.product((0, 1, 2), (1, 40, 64, 80, 128, 200, 256), ((1, 1), (8, 8), (12, 1), (16, 2), (600, 600)),
+                                                                 (1, 7, 64, 5000), (1, 100, 1 << 20), (16, 18), (16, None)):
+        assert 0 < need(io_dtype=io, D=D, Hq=Hq, Hk=Hk, B=B, table_width=width, q=q, block_table=table, num_pages=5000) <= n << shift

@@ -12,8 +12,8 @@
 //   equal runs, whatever the lengths (they are on the device: every block sums them up itself), a run to a block for each head,
 //   or, with the heads' units in the row as well, to one block (make_plan chooses).  A block's run covers the end of one
 //   (sequence, head), some whole ones, and the beginning of another; whole ones are finished in place, the two open ones leave
-//   (m, sum, unnormalised out) in the scratch, which the second kernel joins.  At most two open ones a block: the scratch does
-//   not grow with the batch.  The second kernel is launched so that it is set up while the first still runs.
+//   (m, sum, unnormalised out) in the scratch, which the second kernel joins.  At most two open ones a block, and no
+//   more blocks than the GPU runs at a time: the scratch grows with the work only as long as that has fewer units.  The second kernel is launched so that it is set up while the first still runs.
 // * No shared memory on the way.  With keys as the rows of the first product (S^T = K Q^T) a lane's piece of the A operand is
 //   16 contiguous bytes of two key rows, once the order of the summed dimensions is agreed with Q; for the second
 //   (O^T = V^T P^T) it is 16 contiguous bytes of four value rows, after one byte permutation a register.  So loads go from
@@ -600,6 +600,19 @@ template <typename T, bool VEC> __device__ __forceinline__ float4 load4(const T*
 
 constexpr int any_blocks_per_sm(int DP, int HP) { return DP == 256 ? (HP == 1 ? 3 : 2) : 4; }
 
+// Scratch: (sums, m, l) of two open pieces a block, and what is open.
+constexpr int64_t scratch_bytes(int64_t blocks, int DP, int HP) { return blocks * 2 * HP * (DP * 4 + 8) + blocks * (int64_t)sizeof(Open); }
+constexpr bool scratch_fits() {
+    for (int DP = 64; DP <= 256; DP *= 2) {
+        for (int NT = 1; NT <= 2; ++NT)
+            if (scratch_bytes(kNumSMs * decode_blocks_per_sm(DP, NT), DP, 8 * NT) > VTX_PAGED_DECODE_SCRATCH_MAX && !(DP == 256 && NT == 2)) return false;
+        for (int HP = 1; HP <= 4; HP += 3)
+            if (scratch_bytes(kNumSMs * any_blocks_per_sm(DP, HP), DP, HP) > VTX_PAGED_DECODE_SCRATCH_MAX) return false;
+    }
+    return true;
+}
+static_assert(scratch_fits(), "VTX_PAGED_DECODE_SCRATCH_MAX");
+
 template <typename T, int DP, int HP, bool VEC>
 __global__ void __launch_bounds__(kThreads, any_blocks_per_sm(DP, HP)) decode_any_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int C = DP / 32, PITCH = DP + 4, STEPS = HP == 1 ? 256 / DP : DP == 64 ? 2 : 1;
@@ -825,7 +838,7 @@ Plan make_plan(const vtx_paged_decode_params& p) {
     pl.abreast = groups <= pl.blocks && (pl.blocks % groups * 20 <= pl.blocks || !lines) ? (int)groups : 1;
     pl.blocks -= pl.blocks % pl.abreast;
     pl.slots = (int64_t)pl.blocks * 2 * pl.HP;
-    pl.bytes = pl.slots * (pl.DP * 4 + 8) + (int64_t)pl.blocks * sizeof(Open);
+    pl.bytes = scratch_bytes(pl.blocks, pl.DP, pl.HP);
     return pl;
 }
 
