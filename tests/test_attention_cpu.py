@@ -364,3 +364,13 @@ def test_decode_attention_scratch_maximum():
     for io, D, (Hq, Hk), B, width, q, table in itertools.product((0, 1, 2), (1, 40, 64, 80, 128, 200, 256), ((1, 1), (8, 8), (12, 1), (16, 2), (600, 600)),
                                                                  (1, 7, 64, 5000), (1, 100, 1 << 20), (16, 18), (16, None)):
         assert 0 < need(io_dtype=io, D=D, Hq=Hq, Hk=Hk, B=B, table_width=width, q=q, block_table=table, num_pages=5000) <= n << shift
+
+
+def test_a_sequence_read_back_in_order():
+    """What a later chunk of a prompt attends to: a sequence's pages, flattened."""
+    c = cache()
+    a, b = c.open(), c.open()
+    for n in (6, 5):
+        pos, seq = c.extend([b, a], [n, n + 1])
+        store(c, pos, seq, [100.0 * s + p for p, s in zip(pos.tolist(), seq.tolist())])
+    assert c.k[0][c.pages(a)].flatten(0, 1)[:c.length(a)].flatten().tolist() == [100.0 * a + p for p in range(13)]

@@ -62,8 +62,8 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, e
     A head with a weight [D] is divided by its root mean square first, ``u = w x / sqrt(mean x^2 + eps)``.  Then pair i of
     its first ``rot = 2 * len(inv_freq)`` values turns by ``position * inv_freq[i]``: values (2i, 2i + 1) when
     ``interleaved``, else (i, i + rot / 2); rotated values are multiplied by ``scale``, the others kept.  ``positions`` are
-    int32 or int64, [T], [B, L] or [L] for every batch element; ``inv_freq`` float64 (or float32) on the device, see
-    ``rotary_inv_freq``.  Angles are formed in 64 bits, the rest in fp32, rounded once.  Differentiable in q, k and the
+    int32 or int64 (any sign, below 2^31), [T], [B, L] or [L] for every batch element; ``inv_freq`` float64 (or float32) on the device, see
+    ``rotary_inv_freq``.  Angles are formed and reduced to a turn in 64 bits, the rest in fp32, rounded once.  Differentiable in q, k and the
     weights, once and in reverse mode (a second differentiation raises, as forward mode does); the weights' gradients are
     summed in a fixed order.  D <= 512."""
     qo, ko = ops.qk_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, eps=eps, interleaved=interleaved, scale=scale)
@@ -73,7 +73,7 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, e
 def rotary_append(q, k, v, positions, k_pages, v_pages, block_table, inv_freq=None, q_weight=None, k_weight=None, *,
                   seq_ids=None, eps=1e-6, interleaved=False, scale=1.0):
     """``qk_norm_rotary`` on new tokens, whose keys, and values ``v`` as they are, go to the pages of a cache; returns the
-    queries.  One launch; not differentiable.
+    queries.  One launch; not differentiable (the result is detached, the pools' versions rise).
 
     ``k_pages``, ``v_pages`` [pages, page_size, Hk, D] (any strides but over D) are written in place.  Token t belongs to row
     ``seq_ids[t]`` (int32 [T]; without it there is one token for every row) of ``block_table`` (int32 [sequences, pages of a
@@ -93,7 +93,9 @@ def paged_decode_attention(q, k_pages, v_pages, block_table, seqlens, *, softmax
     Scores are multiplied by ``softmax_scale`` (1 / sqrt(D)); ``window`` > 0 keeps the last so many keys.  A sequence of no
     keys gives zeros and -inf.  ``block_table`` None: contiguous caches [B, keys, Hk, D].  Lengths and table are read on the
     device: the call can be captured and replayed while they change.  Keys that the table gives no page are left out, and
-    ``ops.device_status()`` raises.  Not differentiable.  D <= 256."""
+    ``ops.device_status()`` raises (a sequence that is left none gives zeros and -inf as well).  Scores and sums are fp32; where
+    16-bit values are multiplied on the tensor cores, probabilities enter as head and remainder of their type, off by 2^-16 of
+    themselves at most.  Not differentiable: the result is detached.  D <= 256."""
     out, lse = ops.paged_decode_attention(q, k_pages, v_pages, block_table, seqlens, softmax_scale=softmax_scale, window=window,
                                           want_lse=return_lse)
     return (out, lse) if return_lse else out

@@ -2,11 +2,13 @@
 //
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = exp2(s_j - m),  s_j = log2(e) * softmax_scale * (q . k_j)
 //
-// in one pass over the cache with a running maximum m.  Every key and value is read once for up to 16 query heads, two
-// operations a byte and head: memory bounds it.  Measured (bf16, of the measured copy bandwidth): 64 sequences of 8192-8704
-// keys, 32 heads of 128, 1285-1320 us and one of 1,048,576 keys, 8 heads, 631 us (1.0); 32 sequences of 4000-8000 keys, 64
-// query heads over 8, 126-130 us (0.95); 48 ragged ones, 32 over 8 heads of 64 in fp16, 224 us (0.93); one of 700 keys 8.7 us
-// (a chain of launch, lengths, table, keys, join and join's launch).  What the kernels are built around:
+// in one pass over the cache with a running maximum m.  Every key and value is read once for up to 16 query heads (8 where a head
+// has more than 128 values, 4 on the CUDA cores; beyond, a pass over the cache for each so many), two operations a byte and head:
+// memory bounds it.  Measured (bf16, of the measured copy bandwidth, replayed from a graph; in brackets as a program's calls on
+// changing inputs): 64 sequences of 8192-8704 keys, 32 heads of 128, 1280-1318 us (1.0; 1405, 0.96) and one of 1,048,576 keys, 8
+// heads, 640-666 us (1.0; 682, 0.96); 32 sequences of 4000-8000 keys, 64 query heads over 8, 130 us (0.93); 48 ragged ones, 32
+// over 8 heads of 64 in fp16, 224-236 us (0.88-0.93; 254, 0.82); one of 700 keys 8.8 us (11.6; a chain of launch, lengths, table,
+// keys, join and join's launch).  What the kernels are built around:
 //
 // * Work.  The cache is cut into units of 64 or 128 keys of one key head; the units of all sequences, in a row, are dealt out in
 //   equal runs, whatever the lengths (they are on the device: every block sums them up itself), a run to a block for each head,
@@ -578,8 +580,10 @@ __global__ void __launch_bounds__(kThreads, decode_blocks_per_sm(DP, NT)) decode
 // ---- any type, head size and alignment: fp32 products on the CUDA cores ----------------------------------------------------
 // Eight lanes hold a key, a lane the values 32 i + 4 (lane % 8) .. + 3 of it; a warp works on four keys at a time, each group
 // of eight lanes with a maximum and sums of its own.  Up to four query heads at a time; one alone leaves registers for more
-// keys in flight.  fp32, 16 sequences of 4000-8000 keys, 16 heads of 128: 228 us (1.0); 32 sequences, 32 over 8 heads: 373 us
-// (0.64: issue slots, and one step in flight).
+// keys in flight.  fp32, 16 sequences of 4000-8000 keys, 16 heads of 128: 229 us (1.0); 32 sequences, 16 to 32 over 8 heads:
+// 359-376 us (0.65: issue slots, and one step in flight), 40 to 64 over 8: 676-699 us (0.36: two passes); heads of 64, 32 and 64
+// over 8: 208 and 406 us (0.55, 0.30); of 256, 16 and 32 over 4: 393 and 717 us (0.60, 0.32).  bf16 heads of 44, 16 over 16: 374
+// us (0.22: no 16-byte vectors of eight values, so not the tensor cores).
 template <typename T, bool VEC> __device__ __forceinline__ float4 load4(const T* p, int d, int D) {
     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
     if (VEC) {

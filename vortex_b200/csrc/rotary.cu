@@ -7,14 +7,18 @@
 //   backward, with g = the transposed rotation of dy:  dx = (w g - xh mean(w g xh)) / r,  dw = sum over rows of g xh.
 //
 // Every value is read once and written once, in fp32 between the two, rounded once: memory bounds it, and below some 10^4
-// rows the launch.  The sine and cosine of a (token, pair) are formed once for up to 16 heads, in shared memory.  The angle is
-// formed in 64 bits, as turns with the whole turns taken off, since position * inv_freq in 32 bits is off by 0.03 rad at
-// position 2^20; what is left goes to sincospif.
+// rows the launch.  The vector kernels form the sine and cosine of a (token, pair) once for the heads of a warp, in shared
+// memory: up to four steps of 32 / lanes heads side by side (32 16-bit heads of up to 64 values, 16 of 128, 8 of 256, 4 of 512;
+// half as many in fp32).  The angle is formed in 64 bits, as turns with the whole turns taken off, since position * inv_freq in
+// 32 bits is off by 0.03 rad at position 2^20; what is left, half a turn at most, goes to sincospif as a float.
 //
-// Measured (bf16, heads of 128, of the measured copy bandwidth): 32768 tokens x 64 heads turned in 167 us (0.98); 16384 tokens x
-// 40 heads normed and turned in 68 us (0.75: the norm's two waits for other lanes, and warps of 8 key heads that are short
-// beside their set-up), backward 100 us (0.77: registers, two blocks an SM); 9757 ragged tokens x 48 heads stored in pages in
-// 50 us (0.73); 64 tokens x 64 heads in 2.8 us, stored 3.6 us (the chain position -> table -> store behind the launch).
+// Measured (bf16, heads of 128, of the measured copy bandwidth; replayed from a graph): 32768 tokens x 64 heads turned in 167 us
+// (0.98; 181 as a program's calls on changing inputs, 0.90); 16384 tokens x 40 heads normed and turned in 68 us (0.75: the
+// norm's two waits for other lanes, and warps of 8 key heads that are short beside their set-up), backward 100 us (0.77:
+// registers, two blocks an SM), in fp32 114 and 173 us (0.90, 0.89); 9757 ragged tokens x 48 heads stored in pages in 50 us
+// (0.73); 64 tokens x 64 heads in 2.8 us, stored 3.7 us (the chain position -> table -> store behind the launch).  The general
+// kernels form every angle for every head and read value by value: bf16 heads of 80 with 40 turned, 16384 tokens x 40 heads,
+// 252 us, normed 346, backward 657 (0.13, 0.09, 0.07); fp32 heads of 512, x 10, 194, 227 and 561 us (0.53, 0.45, 0.27).
 #include "attn.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
@@ -478,7 +482,8 @@ __global__ void __launch_bounds__(kThreads, kBwdPerSM) rotary_bwd_kernel(const _
     }
 }
 
-// Any head size and alignment: a warp per (token, head), values one by one.  Pair i, and the kept dimensions behind the
+// Any head size and alignment (heads or rotated parts that are no whole pairs of 16-byte vectors, as 40 of 80 16-bit values, or
+// that have more than 32 of them; rows off 16-byte boundaries): a warp per (token, head), values one by one.  Pair i, and the kept dimensions behind the
 // pairs, belong to lane i % 32 in both passes, which is what lets a row be rewritten in place.
 struct Pairs {
     int half, rot, D, inter;
